@@ -200,6 +200,75 @@ int ogv_layernorm_bwd(const void* dy, const void* x, const float* gamma, const f
                       int M, int C, ogv_dtype dt, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Attention over packed sequences of different lengths (no reference counterpart: the reference's attention,
+ * src/model/grid_attention.py:62-89, takes equal token sets; this is the same softmax(q k^T scale) v for sets of
+ * different sizes laid end to end, with shared key / value heads).
+ *   q, out [Mq][heads][D], k, v [Mk][kv_heads][D] with the given row and head strides (elements, multiples of
+ *   16 bytes; the last dim is contiguous, pointers 16-B aligned); lse fp32 [Mq][heads].
+ *   Sequence b: queries cu_q[b] .. cu_q[b + 1] - 1, keys cu_k[b] .. cu_k[b + 1] - 1 (int32 [B + 1] on the device,
+ *   not decreasing; the first offset is taken as 0, all are clamped to [0, M]).  Any length may be 0.
+ *   causal: key j of a sequence is seen by its query i where j <= i + keys - queries.
+ *   A row that sees no key, and a row behind the last sequence: out 0, lse -inf, gradients 0.
+ * Backward: dout, dq like q; dk, dv like k; out and lse as the forward wrote them.
+ * ws >= the *_ws_bytes query (forward: 0 bytes, may be NULL, unless the keys are split).  Deterministic.
+ * The backward forms the weights again from lse in fp32: a weight's relative error is about 2^-23 |scale q . k|.
+ * A non-finite value in v reaches its own sequence only.  bf16 or fp32, D % 8 == 0, D <= 128, scale > 0.
+ * ------------------------------------------------------------------------------------------- */
+#define OGV_PACKED_TENSORS 8
+typedef struct {
+  int B, Mq, Mk, heads, kv_heads, D, causal;
+  float scale;
+  int64_t row[OGV_PACKED_TENSORS], head[OGV_PACKED_TENSORS]; /* strides of q, k, v, out, dout, dq, dk, dv */
+} ogv_packed_desc;
+size_t ogv_packed_attn_fwd_ws_bytes(const ogv_packed_desc* d, ogv_dtype dt);
+int ogv_packed_attn_fwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* out,
+                        float* lse, void* ws, const ogv_packed_desc* d, ogv_dtype dt, void* stream);
+size_t ogv_packed_attn_bwd_ws_bytes(const ogv_packed_desc* d, ogv_dtype dt);
+int ogv_packed_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
+                        const float* lse, const int* cu_q, const int* cu_k, void* dq, void* dk, void* dv, void* ws,
+                        const ogv_packed_desc* d, ogv_dtype dt, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Rotary positions with several axes on q [M][heads[0]][D] and, with heads[1] > 0, k [M][heads[1]][D] (no
+ * reference counterpart).  Axis x has pairs[x] pairs of numbers; the j-th is turned by
+ * position[m][x] * theta^(-j / pairs[x]).  With P pairs in all, pair p is dims (p, p + P), or (2p, 2p + 1) with
+ * `interleaved`; dims from 2 P on pass unchanged.  inverse: the negative angles (the backward).
+ * positions [M][axes] int32, or fp32 with pos_float.  Outputs may be the inputs themselves with equal strides.
+ * ------------------------------------------------------------------------------------------- */
+#define OGV_ROTARY_AXES 4
+typedef struct {
+  int M, heads[2], D, axes, pairs[OGV_ROTARY_AXES], interleaved, inverse, pos_float;
+  double theta;
+  int64_t row_in[2], head_in[2], row_out[2], head_out[2];
+} ogv_rotary_desc;
+int ogv_axial_rotary(const void* q, void* q_out, const void* k, void* k_out, const void* positions,
+                     const ogv_rotary_desc* d, ogv_dtype dt, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * The end of a residual half-block and the norm that begins the next (no reference counterpart; extends the
+ * x + DropPath(f) and LayerNorm of src/model/Out_Grid_Block.py:98-104 with a norm behind the branch and a gate):
+ *   y = alpha x + rs[m / rps] * gate * N_post(f)        h = N_pre(y)
+ * f, x, y, h [M, C] rows; kinds: none (post: N_post(f) = f; pre: no h), layer, rms; weights and biases fp32 [C],
+ * NULL = 1 / 0; gate fp32 [samples][C] (row m belongs to sample m / (M / samples); samples = 1: per channel),
+ * NULL = 1; rs fp32 [ceil(M / rps)], NULL = 1 (not differentiated).  stats fp32 [M][4] (NULL: no backward).
+ * Backward: dy or dh may be NULL (zero); sums fp32 [5][C] = d gate (samples == 1), d pre_w, d pre_b, d post_w,
+ * d post_b (those of absent parameters are to be ignored); dgate fp32 [samples][C] with samples > 1.  1 <= C <= 8192.
+ * ------------------------------------------------------------------------------------------- */
+typedef enum { OGV_NORM_NONE = 0, OGV_NORM_LAYER = 1, OGV_NORM_RMS = 2 } ogv_norm_kind;
+typedef struct {
+  int M, C, post, pre, samples, rps;
+  float alpha, post_eps, pre_eps;
+} ogv_gated_norm_desc;
+int ogv_gated_norm_fwd(const void* f, const void* x, const float* gate, const float* rs, const float* post_w,
+                       const float* post_b, const float* pre_w, const float* pre_b, void* y, void* h, float* stats,
+                       const ogv_gated_norm_desc* d, ogv_dtype dt, void* stream);
+size_t ogv_gated_norm_bwd_ws_bytes(const ogv_gated_norm_desc* d, ogv_dtype dt);
+int ogv_gated_norm_bwd(const void* dy, const void* dh, const void* f, const void* x, const float* gate,
+                       const float* rs, const float* post_w, const float* post_b, const float* pre_w,
+                       const float* pre_b, const float* stats, void* df, void* dx, float* sums, float* dgate, void* ws,
+                       const ogv_gated_norm_desc* d, ogv_dtype dt, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Dense projection GEMMs on MFMA (1x1 Conv2d / nn.Linear of the hot path:
  * outlook_attention.py:83-88,37-40; grid_attention.py:57-59; Out_Grid_Block.py:18-21).
  *

@@ -1,0 +1,162 @@
+// Shared pieces of the packed-sequence attention kernels (ogv_packed_fwd.hip, ogv_packed_bwd.hip).
+//
+// Rows.  The G = heads / kv_heads query heads that share a key / value head are extra rows of one
+// problem: row r of sequence b and key / value head h is query r / G, head h * G + r % G.  A key /
+// value tile is then read once for the whole group, and a single query still fills G rows.
+//
+// Fragments (32x32 MFMA, lane = 32 * hf + c, hf = lane >> 5, c = lane & 31; a 16-B chunk holds E = 8
+// bf16 or 4 fp32 values):
+//   A / B operand of reduction step kk: row (column) c, chunk 2 * kk + hf.  bf16: one 32x32x16 product.
+//     fp32: four 32x32x2 products, element e of the chunk each.  Both operands are read alike, so the
+//     order of the reduction inside a step does not matter.
+//   C / D: column c, rows 8 * (i / 4) + 4 * hf + i % 4 in register i = 0..15.
+//   A C tile is the B operand of the next product as it stands: register 8 * s + j (bf16) goes to
+//   reduction slot j, so the A operand takes rows 16 * s + 4 * hf + {0..3} and + 8 -- what two
+//   ds_read_b64_tr_b16 of a row-major LDS tile deliver -- and for fp32 register i is one product with
+//   row 8 * (i / 4) + 4 * hf + i % 4.
+//
+// LDS tiles are row-major without padding; 16-B chunk ch of row r sits at ch ^ swz(r).  With RB bytes a
+// row, swz keeps both access shapes free of bank conflicts: 16 rows of one chunk (b128 operand reads) and
+// 4 rows of 64 B (transposed reads).
+#pragma once
+#include "ogv_common.h"
+
+namespace ogv {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((address_space(3))) s16x4 lds_tr_t;
+
+struct PackedArgs {
+  const void *q, *k, *v, *o, *dout;   // o: forward's output (read by the backward)
+  void *out, *dq, *dk, *dv;
+  float *lse, *delta;
+  const int *cu_q, *cu_k;
+  float *part_o, *part_ml;            // split forward: [split][Mq * hq][D] and [split][Mq * hq][2]
+  int B, Mq, Mk, hq, hkv, D, G, causal;
+  unsigned gmagic;                    // ceil(2^32 / G); r / G = umulhi(r, gmagic) for r * G < 2^32
+  int tiles, nsplit;                  // tile slots per key / value head; key splits
+  float scale;
+  long rq, rk, rv, ro, rdo, rdq, rdk, rdv;   // row strides, elements
+  long hsq, hsk, hsv, hso, hsdo, hsdq, hsdk, hsdv;   // head strides, elements
+};
+
+// r / G (G == 1 has no 32-bit magic number)
+__device__ __forceinline__ int group_div(int r, int G, unsigned magic) {
+  return G == 1 ? r : (int)__umulhi((unsigned)r, magic);
+}
+
+template <int RB> __device__ __forceinline__ int swz(int r) {
+  if constexpr (RB % 256 == 0) return ((r & 3) << 2) | ((r >> 2) & 3);
+  else if constexpr (RB % 128 == 0) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  else return (r >> 2) & 3;
+}
+
+template <typename T, int D> struct Frag {
+  static constexpr int E = 16 / sizeof(T);          // elements per 16-B chunk
+  static constexpr int RB = D * (int)sizeof(T);     // bytes per LDS row
+  static constexpr int NC = RB / 16;                // chunks per row
+  static constexpr int KK = NC / 2;                 // reduction steps over D
+};
+
+union Chunk {
+  uint4 u;
+  bf16x8 h;
+  f32x4 f;
+};
+
+__device__ __forceinline__ Chunk zero_chunk() {
+  Chunk c;
+  c.u = make_uint4(0, 0, 0, 0);
+  return c;
+}
+
+// acc += A . B over one reduction step
+template <typename T> __device__ __forceinline__ void mfma_step(const Chunk& a, const Chunk& b, f32x16& acc) {
+  if constexpr (sizeof(T) == 2) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, b.h, acc, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.f[e], b.f[e], acc, 0, 0, 0);
+  }
+}
+
+template <int RB> __device__ __forceinline__ Chunk lds_chunk(const char* tile, int row, int ch) {
+  Chunk c;
+  c.u = *reinterpret_cast<const uint4*>(tile + row * RB + ((ch ^ swz<RB>(row)) << 4));
+  return c;
+}
+
+// B operand of the next product: 16 rows (bf16) of a C tile, registers 8 * s .. 8 * s + 7
+__device__ __forceinline__ Chunk pack8(const f32x16& x, int s) {
+  Chunk c;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c.h[j] = (bf16)x[8 * s + j];
+  return c;
+}
+
+// acc[db] += X^T . Y for one 32-row block of the LDS tile: X is rows row0 .. row0 + 31 of the tile, y the
+// C tile whose rows are the same 32 rows, acc[db] the dims 32 * db .. + 31 (rows) of y's columns.
+template <typename T, int D>
+__device__ __forceinline__ void accum_xt(const char* tile, int row0, const f32x16& y, f32x16 (&acc)[D / 32], int lane) {
+  constexpr int RB = Frag<T, D>::RB;
+  const int hf = lane >> 5;
+  if constexpr (sizeof(T) == 2) {
+    const int fr = lane & 15, part = (lane >> 4) & 1;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const Chunk yb = pack8(y, s);
+      const int row = row0 + 16 * s + 4 * hf + (fr >> 2);
+      const int sw0 = swz<RB>(row), sw1 = swz<RB>(row + 8);
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) {
+        const int ch = db * 4 + part * 2 + ((fr >> 1) & 1), sub = (fr & 1) * 8;
+        union { s16x4 p[2]; bf16x8 h; } a;
+        a.p[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_t*)(tile + row * RB + ((ch ^ sw0) << 4) + sub));
+        a.p[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_t*)(tile + (row + 8) * RB + ((ch ^ sw1) << 4) + sub));
+        acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, yb.h, acc[db], 0, 0, 0);
+      }
+    }
+  } else {
+    const int c = lane & 31;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = row0 + 8 * (i / 4) + 4 * hf + i % 4;
+      const int sw = swz<RB>(row);
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) {
+        const float a = *reinterpret_cast<const float*>(tile + row * RB + (((db * 8 + (c >> 2)) ^ sw) << 4) + (c & 3) * 4);
+        acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, y[i], acc[db], 0, 0, 0);
+      }
+    }
+  }
+}
+
+// Tile slot t of sequence-major tiles of BM rows: the slots of sequence b begin at cu[b] * G / BM + b, which
+// leaves every sequence room for ceil(len * G / BM) tiles, needs no table and bounds their number by
+// M * G / BM + B.  A whole wave searches (64 probes a round).  Offsets are clamped to [0, M], the first one
+// to 0, so a bad offset array cannot lead outside the tensors.
+struct Seq {
+  int b, tile, start, len;
+};
+__device__ __forceinline__ int cu_at(const int* __restrict__ cu, int b, int M) {
+  return b <= 0 ? 0 : min(max(cu[b], 0), M);
+}
+__device__ __forceinline__ Seq find_tile(const int* __restrict__ cu, int B, int M, int G, int BM, int t, int lane) {
+  int lo = 0, n = B;   // the answer is in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 63) >> 6, idx = lo + lane * step;
+    const bool ok = lane * step < n && (int)(((long)cu_at(cu, idx, M) * G) / BM) + idx <= t;
+    const int hits = __popcll(__ballot(ok));
+    const int j = hits > 0 ? hits - 1 : 0;
+    n = min(step, n - j * step);
+    lo += j * step;
+  }
+  Seq s;
+  s.b = __builtin_amdgcn_readfirstlane(lo);
+  s.start = __builtin_amdgcn_readfirstlane(cu_at(cu, s.b, M));
+  s.len = __builtin_amdgcn_readfirstlane(max(cu_at(cu, s.b + 1, M) - s.start, 0));
+  s.tile = t - ((int)(((long)s.start * G) / BM) + s.b);
+  return s;
+}
+
+}  // namespace ogv

@@ -1,0 +1,307 @@
+// Attention over packed sequences of different lengths, forward.
+//
+//   s_rj = scale * q_r . k_j        key j of r's sequence, causal: j <= pos(r) + keys - queries
+//   m_r = max_j s_rj,  l_r = sum_j exp(s_rj - m_r)
+//   o_r = sum_j exp(s_rj - m_r) v_j / l_r,  lse_r = m_r + log(l_r);  no visible key: o_r = 0, lse_r = -inf
+//
+// One pass over the keys with a running maximum and sum.  A wave owns 32 rows; scores are computed
+// transposed (S^T = K Q^T), so a row's scores lie in two lanes and its maximum, sum and rescaling are
+// lane-local but for one exchange, and P^T feeds O^T += V^T P^T from registers.  K and V tiles pass
+// through LDS once per workgroup.  Scores, maximum, sum and O are fp32; P is rounded to bf16 for the second
+// product (relative error 2^-9 per weight, independent from key to key, below the output's own rounding).
+#include "ogv_packed.h"
+
+#include <initializer_list>
+
+namespace ogv {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <typename T, int D, int NW, bool SPLIT>
+__global__ __launch_bounds__(NW * 64) void packed_fwd_kernel(const PackedArgs a) {
+  using F = Frag<T, D>;
+  constexpr int BM = 32 * NW, BN = sizeof(T) == 2 ? 64 : 32, NB = BN / 32, NT = NW * 64;
+  constexpr int RB = F::RB, NC = F::NC, KK = F::KK, E = F::E;
+  __shared__ __attribute__((aligned(16))) char Ks[BN * RB];
+  __shared__ __attribute__((aligned(16))) char Vs[BN * RB];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hf = lane >> 5, c = lane & 31;
+
+  long id;
+  if (!xcd_block((long)a.hkv * a.tiles * a.nsplit, id)) return;
+  const int split = SPLIT ? (int)(id % a.nsplit) : 0;
+  const long ht = SPLIT ? id / a.nsplit : id;
+  const int h = (int)(ht / a.tiles), t = a.tiles - 1 - (int)(ht % a.tiles);
+  const Seq sq = find_tile(a.cu_q, a.B, a.Mq, a.G, BM, t, lane);
+  const int k0 = cu_at(a.cu_k, sq.b, a.Mk), lk = max(cu_at(a.cu_k, sq.b + 1, a.Mk) - k0, 0);
+  const int rows = sq.len * a.G, r0 = sq.tile * BM;
+  // rows behind the last sequence belong to nothing: zeros
+  const int store_rows = sq.b == a.B - 1 ? (a.Mq - sq.start) * a.G : rows;
+  if (r0 >= store_rows) return;
+  const int off = lk - sq.len;
+  int kend = r0 < rows ? lk : 0;
+  if (a.causal && kend) kend = max(0, min(lk, group_div(min(r0 + BM, rows) - 1, a.G, a.gmagic) + off + 1));
+  int kt0 = 0, kt1 = (kend + BN - 1) / BN;
+  if (SPLIT) {
+    const int per = (kt1 + a.nsplit - 1) / a.nsplit;
+    kt0 = min(split * per, kt1);
+    kt1 = min(kt0 + per, kt1);
+  }
+
+  const int r = r0 + wave * 32 + c, pos = group_div(r, a.G, a.gmagic), hg = r - pos * a.G;
+  const bool live = r < rows;
+  const int lim = live ? (a.causal ? min(lk - 1, pos + off) : lk - 1) : -1;   // last visible key
+  Chunk qf[KK];
+  {
+    const T* qp = (const T*)a.q + (long)(sq.start + (live ? pos : 0)) * a.rq + (long)(h * a.G + hg) * a.hsq;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      const int d = (2 * kk + hf) * E;
+      qf[kk] = zero_chunk();
+      if (live && d < a.D) qf[kk].u = *reinterpret_cast<const uint4*>(qp + d);
+    }
+  }
+  f32x16 o[D / 32];
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) o[db] = f32x16{};
+  float m = -INFINITY, l = 0.f;   // m: of q . k, before the scale; l: this lane's half of the row
+  const float c2 = a.scale * LOG2E;
+  const T* kb = (const T*)a.k + (long)k0 * a.rk + (long)h * a.hsk;
+  const T* vb = (const T*)a.v + (long)k0 * a.rv + (long)h * a.hsv;
+
+  for (int kt = kt0; kt < kt1; ++kt) {
+    const int key0 = kt * BN;
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < (BN * NC + NT - 1) / NT; ++n) {
+      const int idx = tid + n * NT;
+      if (BN * NC % NT == 0 || idx < BN * NC) {
+        const int row = idx / NC, ch = idx - row * NC;
+        const bool ok = key0 + row < lk && ch * E < a.D;
+        Chunk kc = zero_chunk(), vc = zero_chunk();
+        if (ok) {
+          kc.u = *reinterpret_cast<const uint4*>(kb + (long)(key0 + row) * a.rk + ch * E);
+          vc.u = *reinterpret_cast<const uint4*>(vb + (long)(key0 + row) * a.rv + ch * E);
+        }
+        const int at = row * RB + ((ch ^ swz<RB>(row)) << 4);
+        *reinterpret_cast<uint4*>(Ks + at) = kc.u;
+        *reinterpret_cast<uint4*>(Vs + at) = vc.u;
+      }
+    }
+    __syncthreads();
+    f32x16 s[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      s[nb] = f32x16{};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) mfma_step<T>(lds_chunk<RB>(Ks, nb * 32 + c, 2 * kk + hf), qf[kk], s[nb]);
+    }
+    if (!__all(key0 + BN - 1 <= lim)) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (key0 + nb * 32 + 8 * (i / 4) + 4 * hf + i % 4 > lim) s[nb][i] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[nb][i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float mn = fmaxf(m, mx), mz = mn == -INFINITY ? 0.f : mn;   // nothing visible yet: weights exp2(-inf) = 0
+    const float corr = __builtin_amdgcn_exp2f((m - mz) * c2);
+    float mu = mz * c2;
+    m = mn;
+    l *= corr;
+    // exp2(s * c2 - mu) in one fma: mu's rounding is the same factor in every weight of the row and cancels, unless
+    // it is large itself; then the maximum is subtracted first
+    if (__any(fabsf(mu) > 16777216.f)) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[nb][i] -= mz;
+      mu = 0.f;
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[nb][i], c2, -mu));
+        s[nb][i] = p;
+        l += p;
+      }
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[db][i] *= corr;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) accum_xt<T, D>(Vs, nb * 32, s[nb], o, lane);
+  }
+
+  l += __shfl_xor(l, 32, 64);
+  if (r >= store_rows) return;
+  const long orow = (long)(sq.start + pos) * a.hq + h * a.G + hg;   // row of the [Mq * hq] outputs
+  if (SPLIT) {   // unnormalised partials, joined by packed_join_kernel
+    float* po = a.part_o + ((long)split * a.Mq * a.hq + orow) * a.D;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = db * 32 + 8 * g + 4 * hf;
+        if (d < a.D) *reinterpret_cast<float4*>(po + d) = make_float4(o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]);
+      }
+    if (hf == 0) {
+      float* ml = a.part_ml + 2 * ((long)split * a.Mq * a.hq + orow);
+      ml[0] = m;
+      ml[1] = l;
+    }
+    return;
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);   // (NaN stays NaN)
+  T* op = (T*)a.out + (long)(sq.start + pos) * a.ro + (long)(h * a.G + hg) * a.hso;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = db * 32 + 8 * g + 4 * hf;
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = o[db][4 * g + e] * inv;
+      if (d < a.D) store_vec<T, 4>(op + d, x);
+    }
+  if (hf == 0) a.lse[orow] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+}
+
+// out = sum_s w_s o_s / sum_s w_s l_s, w_s = exp(scale (m_s - max m)), over the key splits, in split order
+template <typename T>
+__global__ __launch_bounds__(256) void packed_join_kernel(const PackedArgs a) {
+  const int per = a.D / 4;
+  const long n = (long)a.Mq * a.hq * per, idx = (long)blockIdx.x * 256 + threadIdx.x;
+  if (idx >= n) return;
+  const long row = idx / per, R = (long)a.Mq * a.hq;
+  const int d = (int)(idx - row * per) * 4;
+  float m = -INFINITY;
+  for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, a.part_ml[2 * (s * R + row)]);
+  const float mu = m == -INFINITY ? 0.f : m;
+  const float c2 = a.scale * LOG2E;
+  float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float w = __builtin_amdgcn_exp2f((a.part_ml[2 * (s * R + row)] - mu) * c2);
+    l += w * a.part_ml[2 * (s * R + row) + 1];
+    const float4 p = *reinterpret_cast<const float4*>(a.part_o + (s * R + row) * a.D + d);
+    x[0] += w * p.x, x[1] += w * p.y, x[2] += w * p.z, x[3] += w * p.w;
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] *= inv;
+  const long q = row / a.hq;
+  store_vec<T, 4>((T*)a.out + q * a.ro + (row - q * a.hq) * a.hso + d, x);
+  if (d == 0) a.lse[row] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+}
+
+struct FwdPlan {
+  int nw, tiles, nsplit;
+};
+
+// Shortest sequences that fill four waves' rows on average get them, others one wave per workgroup;
+// the keys are split while the workgroups would not fill the 256 CUs.
+static FwdPlan fwd_plan(const ogv_packed_desc* d) {
+  FwdPlan p;
+  const long rows = (long)d->Mq * (d->heads / d->kv_heads);
+  p.nw = rows >= 96L * d->B ? 4 : 1;
+  p.tiles = (int)(rows / (32 * p.nw)) + d->B;
+  const long blocks = (long)p.tiles * d->kv_heads, keys = d->Mk / d->B;
+  long n = blocks >= 512 ? 1 : 1024 / (blocks > 0 ? blocks : 1);
+  const long most = keys / 256;   // at least 256 keys to a split
+  if (n > most) n = most;
+  p.nsplit = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+  return p;
+}
+
+template <typename T, int D>
+static void fwd_launch(const FwdPlan& p, const PackedArgs& a, hipStream_t s) {
+  const unsigned nb = xcd_grid((long)a.hkv * p.tiles * p.nsplit);
+  if (p.nsplit > 1) {
+    if (p.nw == 4) packed_fwd_kernel<T, D, 4, true><<<nb, 256, 0, s>>>(a);
+    else packed_fwd_kernel<T, D, 1, true><<<nb, 64, 0, s>>>(a);
+    packed_join_kernel<T><<<cdiv((long)a.Mq * a.hq * (a.D / 4), 256), 256, 0, s>>>(a);
+  } else {
+    if (p.nw == 4) packed_fwd_kernel<T, D, 4, false><<<nb, 256, 0, s>>>(a);
+    else packed_fwd_kernel<T, D, 1, false><<<nb, 64, 0, s>>>(a);
+  }
+}
+
+int packed_check(const char* what, const ogv_packed_desc* d, ogv_dtype dt) {
+  OGV_REQUIRE(d, "%s: null descriptor", what);
+  OGV_REQUIRE(dt == OGV_F32 || dt == OGV_BF16, "%s: bad dtype %d", what, (int)dt);
+  OGV_REQUIRE(d->B > 0 && d->Mq > 0 && d->Mk >= 0, "%s: bad shape B=%d Mq=%d Mk=%d", what, d->B, d->Mq, d->Mk);
+  OGV_REQUIRE(d->heads > 0 && d->kv_heads > 0 && d->heads % d->kv_heads == 0,
+              "%s: heads=%d must be a multiple of kv_heads=%d", what, d->heads, d->kv_heads);
+  OGV_REQUIRE(d->D >= 8 && d->D <= 128 && d->D % 8 == 0, "%s: head_dim=%d unsupported (need 8 <= D <= 128, D %% 8 == 0)",
+              what, d->D);
+  OGV_REQUIRE(d->scale > 0.f && __builtin_isfinite(d->scale), "%s: scale must be positive and finite", what);
+  const long G = d->heads / d->kv_heads, most = 1L << 30;
+  OGV_REQUIRE((long)d->Mq * G * G < 4 * most && (long)d->Mq * G < most && (long)d->Mk < most && d->B < most / 2,
+              "%s: too many rows (Mq=%d, group %ld, Mk=%d)", what, d->Mq, G, d->Mk);
+  const long grid = most * 2 - 8;
+  OGV_REQUIRE(((long)d->Mq * G / 32 + d->B) * d->kv_heads < grid && ((long)d->Mk / 32 + d->B) * d->kv_heads < grid,
+              "%s: grid too large", what);
+  const long al = 16 / (dt == OGV_BF16 ? 2 : 4);
+  for (int i = 0; i < OGV_PACKED_TENSORS; ++i) {
+    OGV_REQUIRE(d->row[i] >= 0 && d->head[i] >= 0 && d->row[i] % al == 0 && d->head[i] % al == 0,
+                "%s: stride %d (row %lld, head %lld) must be non-negative multiples of 16 bytes", what, i,
+                (long long)d->row[i], (long long)d->head[i]);
+  }
+  return OGV_OK;
+}
+
+void packed_args(const ogv_packed_desc* d, PackedArgs& a) {
+  a = PackedArgs{};
+  a.B = d->B, a.Mq = d->Mq, a.Mk = d->Mk, a.hq = d->heads, a.hkv = d->kv_heads, a.D = d->D;
+  a.G = d->heads / d->kv_heads, a.causal = d->causal, a.scale = d->scale;
+  a.gmagic = (unsigned)(((1ull << 32) + a.G - 1) / a.G);
+  const int64_t *r = d->row, *h = d->head;
+  a.rq = r[0], a.rk = r[1], a.rv = r[2], a.ro = r[3], a.rdo = r[4], a.rdq = r[5], a.rdk = r[6], a.rdv = r[7];
+  a.hsq = h[0], a.hsk = h[1], a.hsv = h[2], a.hso = h[3], a.hsdo = h[4], a.hsdq = h[5], a.hsdk = h[6], a.hsdv = h[7];
+}
+
+bool aligned16(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if ((uintptr_t)p & 15) return false;
+  return true;
+}
+
+}  // namespace ogv
+
+using namespace ogv;
+
+extern "C" size_t ogv_packed_attn_fwd_ws_bytes(const ogv_packed_desc* d, ogv_dtype dt) {
+  if (packed_check("ogv_packed_attn_fwd_ws_bytes", d, dt) != OGV_OK) return 0;
+  const FwdPlan p = fwd_plan(d);
+  return p.nsplit == 1 ? 0 : (size_t)p.nsplit * d->Mq * d->heads * (d->D + 2) * sizeof(float);
+}
+
+extern "C" int ogv_packed_attn_fwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k,
+                                   void* out, float* lse, void* ws, const ogv_packed_desc* d, ogv_dtype dt,
+                                   void* stream) {
+  if (int rc = packed_check("ogv_packed_attn_fwd", d, dt)) return rc;
+  OGV_REQUIRE(q && cu_q && cu_k && out && lse && (d->Mk == 0 || (k && v)), "ogv_packed_attn_fwd: null pointer");
+  const FwdPlan p = fwd_plan(d);
+  OGV_REQUIRE(p.nsplit == 1 || ws, "ogv_packed_attn_fwd: null workspace");
+  OGV_REQUIRE(aligned16({q, k, v, out, ws}), "ogv_packed_attn_fwd: pointers must be 16-byte aligned");
+  PackedArgs a;
+  packed_args(d, a);
+  a.q = q, a.k = k, a.v = v, a.cu_q = cu_q, a.cu_k = cu_k, a.out = out, a.lse = lse;
+  a.tiles = p.tiles, a.nsplit = p.nsplit;
+  a.part_o = (float*)ws;
+  a.part_ml = (float*)ws + (size_t)p.nsplit * d->Mq * d->heads * d->D;
+  hipStream_t s = as_stream(stream);
+#define OGV_FWD(T)                                      \
+  if (d->D <= 32) fwd_launch<T, 32>(p, a, s);           \
+  else if (d->D <= 64) fwd_launch<T, 64>(p, a, s);      \
+  else if (d->D <= 96) fwd_launch<T, 96>(p, a, s);      \
+  else fwd_launch<T, 128>(p, a, s);
+  if (dt == OGV_BF16) { OGV_FWD(bf16) } else { OGV_FWD(float) }
+#undef OGV_FWD
+  return check_launch("ogv_packed_attn_fwd");
+}

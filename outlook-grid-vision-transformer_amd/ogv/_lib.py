@@ -62,6 +62,25 @@ class CopySeg(ctypes.Structure):
     _fields_ = [("src", _p), ("dst", _p), ("numel", ctypes.c_longlong)]
 
 
+class PackedDesc(ctypes.Structure):
+    _fields_ = [("B", _i), ("Mq", _i), ("Mk", _i), ("heads", _i), ("kv_heads", _i), ("D", _i), ("causal", _i),
+                ("scale", _f), ("row", ctypes.c_int64 * 8), ("head", ctypes.c_int64 * 8)]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [("M", _i), ("heads", _i * 2), ("D", _i), ("axes", _i), ("pairs", _i * 4), ("interleaved", _i),
+                ("inverse", _i), ("pos_float", _i), ("theta", ctypes.c_double), ("row_in", ctypes.c_int64 * 2),
+                ("head_in", ctypes.c_int64 * 2), ("row_out", ctypes.c_int64 * 2), ("head_out", ctypes.c_int64 * 2)]
+
+
+class GatedNormDesc(ctypes.Structure):
+    _fields_ = [("M", _i), ("C", _i), ("post", _i), ("pre", _i), ("samples", _i), ("rps", _i), ("alpha", _f),
+                ("post_eps", _f), ("pre_eps", _f)]
+
+
+_PKD = ctypes.POINTER(PackedDesc)
+_PRD = ctypes.POINTER(RotaryDesc)
+_PND = ctypes.POINTER(GatedNormDesc)
 _PD = ctypes.POINTER(MBConvDesc)
 _PCD = ctypes.POINTER(ConvBNDesc)
 _PCP = ctypes.POINTER(ConvBNParams)
@@ -90,6 +109,14 @@ SIGNATURES = {
     "ogv_outlook_agg_bwd": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p]),
     "ogv_grid_attn_fwd": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _f, _i, _p]),
     "ogv_grid_attn_bwd": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _f, _i, _p]),
+    "ogv_packed_attn_fwd_ws_bytes": (_sz, [_PKD, _i]),
+    "ogv_packed_attn_fwd": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _PKD, _i, _p]),
+    "ogv_packed_attn_bwd_ws_bytes": (_sz, [_PKD, _i]),
+    "ogv_packed_attn_bwd": (_i, [_p] * 12 + [_PKD, _i, _p]),
+    "ogv_axial_rotary": (_i, [_p, _p, _p, _p, _p, _PRD, _i, _p]),
+    "ogv_gated_norm_fwd": (_i, [_p] * 11 + [_PND, _i, _p]),
+    "ogv_gated_norm_bwd_ws_bytes": (_sz, [_PND, _i]),
+    "ogv_gated_norm_bwd": (_i, [_p] * 16 + [_PND, _i, _p]),
     "ogv_layernorm_fwd": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _f, _i, _p]),
     "ogv_layernorm_bwd_ws_bytes": (_sz, [_i, _i]),
     "ogv_layernorm_bwd": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _p]),

@@ -11,6 +11,7 @@ import torch
 import torch.nn as nn
 
 from . import functional as OF
+from . import packed as PK
 
 
 def act_name(mod: nn.Module):
@@ -113,6 +114,57 @@ class LayerNorm(nn.LayerNorm):
         x2d = x.to(OF.compute_dtype(x)).reshape(-1, x.shape[-1])
         y, r = OF.layer_norm_rows_pair(x2d, self.weight, self.bias, self.eps)
         return y.view(x.shape), r.view(x.shape)
+
+
+class GatedResidualNorm(nn.Module):
+    """The end of a residual half-block and the norm that begins the next one, on [rows, dim]:
+    y = alpha * residual + row_scale * gate * N_post(branch), h = N_pre(y) -> (y, h) (ogv.packed.gated_residual_norm).
+    post_norm / pre_norm: "layer", "rms" or None; gate_init: the per-channel gate's first value, None = no gate."""
+
+    def __init__(self, dim: int, post_norm=None, pre_norm="layer", gate_init=None, alpha: float = 1.0, eps: float = 1e-5):
+        super().__init__()
+        self.post_norm, self.pre_norm, self.alpha, self.eps = post_norm, pre_norm, float(alpha), float(eps)
+
+        def affine(kind):
+            return (nn.Parameter(torch.ones(dim)) if PK.NORMS[kind] else None,
+                    nn.Parameter(torch.zeros(dim)) if kind == "layer" else None)
+
+        self.post_weight, self.post_bias = affine(post_norm)
+        self.pre_weight, self.pre_bias = affine(pre_norm)
+        self.gate = nn.Parameter(torch.full((dim,), float(gate_init))) if gate_init is not None else None
+
+    def forward(self, branch, residual, row_scale=None, rps=1):
+        dt = OF.compute_dtype(branch)
+        return PK.gated_residual_norm(branch.to(dt), residual.to(dt), gate=self.gate, row_scale=row_scale, rps=rps,
+                                      alpha=self.alpha, post_norm=self.post_norm, post_weight=self.post_weight,
+                                      post_bias=self.post_bias, pre_norm=self.pre_norm, pre_weight=self.pre_weight,
+                                      pre_bias=self.pre_bias, post_eps=self.eps, pre_eps=self.eps)
+
+
+class PackedSelfAttention(nn.Module):
+    """Self-attention of sequences of different lengths packed end to end: [rows, dim] -> [rows, dim], with shared
+    key / value heads and, with `sections`, rotary positions (ogv.packed.rotary_attention_rows)."""
+
+    def __init__(self, dim: int, num_heads: int, num_kv_heads=None, qkv_bias: bool = True, sections=None,
+                 theta: float = 10000.0, causal: bool = False):
+        super().__init__()
+        if num_heads <= 0 or dim % num_heads:
+            raise ValueError(f"dim ({dim}) must be divisible by num_heads ({num_heads})")
+        self.num_heads, self.num_kv_heads = num_heads, num_heads if num_kv_heads is None else num_kv_heads
+        if self.num_kv_heads <= 0 or num_heads % self.num_kv_heads:
+            raise ValueError(f"num_heads ({num_heads}) must be a multiple of num_kv_heads ({num_kv_heads})")
+        self.sections, self.theta, self.causal = sections, float(theta), bool(causal)
+        self.qkv = Linear(dim, dim // num_heads * (num_heads + 2 * self.num_kv_heads), bias=qkv_bias)
+        self.proj = Linear(dim, dim)
+
+    def forward(self, x, cu, positions=None, residual=None, row_scale=None, rps=None):
+        """cu: int32 [sequences + 1] row offsets on the device; positions [rows, axes] (with sections); residual /
+        row_scale / rps: as Linear's, in the output projection's epilogue."""
+        if x.ndim != 2:
+            raise ValueError(f"PackedSelfAttention expects packed rows [rows, dim], got {tuple(x.shape)}")
+        out = PK.rotary_attention_rows(self.qkv(x), cu, self.num_heads, self.num_kv_heads, positions=positions,
+                                       sections=self.sections, theta=self.theta, causal=self.causal)
+        return self.proj(out, residual=residual, row_scale=row_scale, rps=rps)
 
 
 class BatchNorm2d(nn.BatchNorm2d):
