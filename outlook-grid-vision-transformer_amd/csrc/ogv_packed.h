@@ -86,6 +86,50 @@ template <int RB> __device__ __forceinline__ Chunk lds_chunk(const char* tile, i
   return c;
 }
 
+// Copies ROWS rows of a strided tensor into an LDS tile, straight from global memory to LDS (no registers): one
+// instruction of a wave fills 64 consecutive chunks, so the swizzle is in the addresses that the lanes read.  Rows past
+// the last one repeat it and chunks past the head repeat the first: whoever uses the tile masks their products.
+// Offsets inside a tile are 32-bit (row strides are below 2^24 elements), the tile's base is a uniform pointer.
+template <typename T, int D, int ROWS, int NW> struct TileCopy {
+  using F = Frag<T, D>;
+  static constexpr int NI = ROWS * F::NC / (64 * NW);
+  static_assert(ROWS * F::NC % (64 * NW) == 0, "whole instructions");
+  unsigned off[NI];   // of this lane's chunks: row * stride + chunk, bytes
+  static __device__ __forceinline__ unsigned place(int slot, int last, int Dlive, long stride) {
+    const int row = slot / F::NC, ch = (slot - row * F::NC) ^ swz<F::RB>(row);
+    return (unsigned)min(row, last) * (unsigned)(stride * sizeof(T)) + (ch * F::E < Dlive ? ch * 16 : 0);
+  }
+  __device__ __forceinline__ void init(int wave, int lane, int Dlive, long stride) {
+#pragma unroll
+    for (int n = 0; n < NI; ++n) off[n] = place((n * NW + wave) * 64 + lane, ROWS, Dlive, stride);
+  }
+  // rows 0 .. ROWS - 1 behind base, of which `left` >= 1 exist
+  __device__ __forceinline__ void load(const T* base, long stride, int left, char* tile, int wave, int lane, int Dlive) const {
+    const char* b = reinterpret_cast<const char*>(base);
+    if (left >= ROWS) {
+#pragma unroll
+      for (int n = 0; n < NI; ++n) issue(b + off[n], tile + (n * NW + wave) * 1024);
+    } else {
+#pragma unroll
+      for (int n = 0; n < NI; ++n)
+        issue(b + place((n * NW + wave) * 64 + lane, left - 1, Dlive, stride), tile + (n * NW + wave) * 1024);
+    }
+  }
+  static __device__ __forceinline__ void issue(const char* g, char* l) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+                                     (__attribute__((address_space(3))) void*)l, 16, 0, 0);
+  }
+};
+
+// Keeps the compiler from running a wave-uniform branch's body always and selecting its results.
+__device__ __forceinline__ void rare_branch() { asm volatile(""); }
+
+// This wave's copies to LDS are done; then everybody's are.
+__device__ __forceinline__ void tiles_ready() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
 // B operand of the next product: 16 rows (bf16) of a C tile, registers 8 * s .. 8 * s + 7
 __device__ __forceinline__ Chunk pack8(const f32x16& x, int s) {
   Chunk c;

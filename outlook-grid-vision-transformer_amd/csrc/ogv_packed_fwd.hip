@@ -17,14 +17,78 @@ namespace ogv {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
+// One tile of keys: scores, running maximum and sum, O += P V.
+template <typename T, int D, int NB>
+__device__ __forceinline__ void fwd_tile(const char* Ks, const char* Vs, const Chunk (&qf)[Frag<T, D>::KK], f32x16 (&o)[D / 32],
+                                         float& m, float& l, int key0, int lim, float c2, float grow, int lane) {
+  constexpr int KK = Frag<T, D>::KK, RB = Frag<T, D>::RB;
+  const int hf = lane >> 5, c = lane & 31;
+  f32x16 s[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    s[nb] = f32x16{};
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) mfma_step<T>(lds_chunk<RB>(Ks, nb * 32 + c, 2 * kk + hf), qf[kk], s[nb]);
+  }
+  if (!__all(key0 + NB * 32 - 1 <= lim)) {
+    rare_branch();
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (key0 + nb * 32 + 8 * (i / 4) + 4 * hf + i % 4 > lim) s[nb][i] = -INFINITY;
+  }
+  float mx = s[0][0];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[nb][i]);
+  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+  // The reference of the weights moves only where a row's maximum passed it by more than 2^8 (in weight): until
+  // then weights up to 2^8 are as exact in fp32 and bf16 as those up to 1, and O need not be rescaled.  Each row
+  // decides for itself, so its result does not depend on the rows beside it.
+  if (__any(mx > m + grow)) {
+    rare_branch();
+    const float mn = mx > m + grow ? mx : m, mz = mn == -INFINITY ? 0.f : mn;
+    const float corr = __builtin_amdgcn_exp2f((m - mz) * c2);
+    m = mn;
+    l *= corr;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[db][i] *= corr;
+  }
+  const float mz = m == -INFINITY ? 0.f : m;   // nothing visible yet: every weight is exp2(-inf) = 0
+  float mu = mz * c2;
+  // exp2(s * c2 - mu) in one fma: mu's rounding is the same factor in every weight of the row and cancels, unless
+  // it is large itself; then the reference is subtracted first
+  if (__any(fabsf(mu) > 16777216.f)) {
+    rare_branch();
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[nb][i] -= mz;
+    mu = 0.f;
+  }
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(s[nb][i], c2, -mu));
+      s[nb][i] = p;
+      l += p;
+    }
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) accum_xt<T, D>(Vs, nb * 32, s[nb], o, lane);
+}
+
 template <typename T, int D, int NW, bool SPLIT>
-__global__ __launch_bounds__(NW * 64) void packed_fwd_kernel(const PackedArgs a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_fwd_kernel(const PackedArgs a) {
   using F = Frag<T, D>;
-  constexpr int BM = 32 * NW, BN = sizeof(T) == 2 ? 64 : 32, NB = BN / 32, NT = NW * 64;
-  constexpr int RB = F::RB, NC = F::NC, KK = F::KK, E = F::E;
-  __shared__ __attribute__((aligned(16))) char Ks[BN * RB];
-  __shared__ __attribute__((aligned(16))) char Vs[BN * RB];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hf = lane >> 5, c = lane & 31;
+  constexpr int BM = 32 * NW, BN = sizeof(T) == 2 && NW > 1 ? 64 : 32, NB = BN / 32;
+  constexpr int RB = F::RB, KK = F::KK, E = F::E;
+  __shared__ __attribute__((aligned(16))) char K0[BN * RB], V0[BN * RB], K1[BN * RB], V1[BN * RB];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5, c = lane & 31;
 
   long id;
   if (!xcd_block((long)a.hkv * a.tiles * a.nsplit, id)) return;
@@ -32,7 +96,8 @@ __global__ __launch_bounds__(NW * 64) void packed_fwd_kernel(const PackedArgs a)
   const long ht = SPLIT ? id / a.nsplit : id;
   const int h = (int)(ht / a.tiles), t = a.tiles - 1 - (int)(ht % a.tiles);
   const Seq sq = find_tile(a.cu_q, a.B, a.Mq, a.G, BM, t, lane);
-  const int k0 = cu_at(a.cu_k, sq.b, a.Mk), lk = max(cu_at(a.cu_k, sq.b + 1, a.Mk) - k0, 0);
+  const int k0 = __builtin_amdgcn_readfirstlane(cu_at(a.cu_k, sq.b, a.Mk));
+  const int lk = __builtin_amdgcn_readfirstlane(max(cu_at(a.cu_k, sq.b + 1, a.Mk) - k0, 0));
   const int rows = sq.len * a.G, r0 = sq.tile * BM;
   // rows behind the last sequence belong to nothing: zeros
   const int store_rows = sq.b == a.B - 1 ? (a.Mq - sq.start) * a.G : rows;
@@ -46,6 +111,17 @@ __global__ __launch_bounds__(NW * 64) void packed_fwd_kernel(const PackedArgs a)
     kt0 = min(split * per, kt1);
     kt1 = min(kt0 + per, kt1);
   }
+
+  const T* kb = (const T*)a.k + (long)k0 * a.rk + (long)h * a.hsk;
+  const T* vb = (const T*)a.v + (long)k0 * a.rv + (long)h * a.hsv;
+  TileCopy<T, D, BN, NW> kc, vc;
+  kc.init(wave, lane, a.D, a.rk);
+  vc.init(wave, lane, a.D, a.rv);
+  auto stage = [&](int kt, char* Ks, char* Vs) {
+    kc.load(kb + (long)kt * BN * a.rk, a.rk, lk - kt * BN, Ks, wave, lane, a.D);
+    vc.load(vb + (long)kt * BN * a.rv, a.rv, lk - kt * BN, Vs, wave, lane, a.D);
+  };
+  if (kt0 < kt1) stage(kt0, K0, V0);
 
   const int r = r0 + wave * 32 + c, pos = group_div(r, a.G, a.gmagic), hg = r - pos * a.G;
   const bool live = r < rows;
@@ -64,78 +140,17 @@ __global__ __launch_bounds__(NW * 64) void packed_fwd_kernel(const PackedArgs a)
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) o[db] = f32x16{};
   float m = -INFINITY, l = 0.f;   // m: of q . k, before the scale; l: this lane's half of the row
-  const float c2 = a.scale * LOG2E;
-  const T* kb = (const T*)a.k + (long)k0 * a.rk + (long)h * a.hsk;
-  const T* vb = (const T*)a.v + (long)k0 * a.rv + (long)h * a.hsv;
+  const float c2 = a.scale * LOG2E, grow = 8.f / c2;
 
-  for (int kt = kt0; kt < kt1; ++kt) {
-    const int key0 = kt * BN;
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < (BN * NC + NT - 1) / NT; ++n) {
-      const int idx = tid + n * NT;
-      if (BN * NC % NT == 0 || idx < BN * NC) {
-        const int row = idx / NC, ch = idx - row * NC;
-        const bool ok = key0 + row < lk && ch * E < a.D;
-        Chunk kc = zero_chunk(), vc = zero_chunk();
-        if (ok) {
-          kc.u = *reinterpret_cast<const uint4*>(kb + (long)(key0 + row) * a.rk + ch * E);
-          vc.u = *reinterpret_cast<const uint4*>(vb + (long)(key0 + row) * a.rv + ch * E);
-        }
-        const int at = row * RB + ((ch ^ swz<RB>(row)) << 4);
-        *reinterpret_cast<uint4*>(Ks + at) = kc.u;
-        *reinterpret_cast<uint4*>(Vs + at) = vc.u;
-      }
-    }
-    __syncthreads();
-    f32x16 s[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      s[nb] = f32x16{};
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) mfma_step<T>(lds_chunk<RB>(Ks, nb * 32 + c, 2 * kk + hf), qf[kk], s[nb]);
-    }
-    if (!__all(key0 + BN - 1 <= lim)) {
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (key0 + nb * 32 + 8 * (i / 4) + 4 * hf + i % 4 > lim) s[nb][i] = -INFINITY;
-    }
-    float mx = s[0][0];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[nb][i]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float mn = fmaxf(m, mx), mz = mn == -INFINITY ? 0.f : mn;   // nothing visible yet: weights exp2(-inf) = 0
-    const float corr = __builtin_amdgcn_exp2f((m - mz) * c2);
-    float mu = mz * c2;
-    m = mn;
-    l *= corr;
-    // exp2(s * c2 - mu) in one fma: mu's rounding is the same factor in every weight of the row and cancels, unless
-    // it is large itself; then the maximum is subtracted first
-    if (__any(fabsf(mu) > 16777216.f)) {
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[nb][i] -= mz;
-      mu = 0.f;
-    }
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[nb][i], c2, -mu));
-        s[nb][i] = p;
-        l += p;
-      }
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[db][i] *= corr;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) accum_xt<T, D>(Vs, nb * 32, s[nb], o, lane);
+  // two tiles of LDS: the next tile is under way while this one is used
+  for (int kt = kt0; kt < kt1; kt += 2) {
+    tiles_ready();
+    if (kt + 1 < kt1) stage(kt + 1, K1, V1);
+    fwd_tile<T, D, NB>(K0, V0, qf, o, m, l, kt * BN, lim, c2, grow, lane);
+    if (kt + 1 >= kt1) break;
+    tiles_ready();
+    if (kt + 2 < kt1) stage(kt + 2, K0, V0);
+    fwd_tile<T, D, NB>(K1, V1, qf, o, m, l, (kt + 1) * BN, lim, c2, grow, lane);
   }
 
   l += __shfl_xor(l, 32, 64);
@@ -248,6 +263,7 @@ int packed_check(const char* what, const ogv_packed_desc* d, ogv_dtype dt) {
               "%s: grid too large", what);
   const long al = 16 / (dt == OGV_BF16 ? 2 : 4);
   for (int i = 0; i < OGV_PACKED_TENSORS; ++i) {
+    OGV_REQUIRE(d->row[i] < (1 << 24), "%s: row stride %d = %lld is too large (below 2^24 elements)", what, i, (long long)d->row[i]);
     OGV_REQUIRE(d->row[i] >= 0 && d->head[i] >= 0 && d->row[i] % al == 0 && d->head[i] % al == 0,
                 "%s: stride %d (row %lld, head %lld) must be non-negative multiples of 16 bytes", what, i,
                 (long long)d->row[i], (long long)d->head[i]);

@@ -13,115 +13,127 @@ call the C-ABI (ogv_packed_attn_*, ogv_axial_rotary, ogv_gated_norm_*).
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
 
 from . import _lib
 from ._lib import OGV_BF16, OGV_F32, GatedNormDesc, PackedDesc, RotaryDesc, check
-from .functional import _ptr, _vp, f32
+from .functional import f32
 
 NORMS = {None: 0, "none": 0, "layer": 1, "rms": 2}
 
-
-def _need(ok, what, exc=ValueError):
-    if not ok:
-        raise exc(what)
+# Small calls are bound by the host, so what depends on sizes alone (the C-ABI's descriptors and workspace sizes) is
+# looked up by value, the device is only switched where it differs, and calls without gradients skip autograd.
 
 
-def _dtype(what, *ts):
+def _dtype(what, first, *ts):
     """The C-ABI's element type of tensors that must agree in it."""
-    t = ts[0].dtype
-    _need(t in (torch.bfloat16, torch.float32), f"{what}: float32 or bfloat16 activations, got {t}", TypeError)
-    for o in ts[1:]:
-        _need(o is None or o.dtype == t, f"{what}: mixed activation types {t} and {None if o is None else o.dtype}", TypeError)
-    return OGV_BF16 if t == torch.bfloat16 else OGV_F32
+    t = first.dtype
+    if t is not torch.bfloat16 and t is not torch.float32:
+        raise TypeError(f"{what}: float32 or bfloat16 activations, got {t}")
+    for o in ts:
+        if o is not None and o.dtype is not t:
+            raise TypeError(f"{what}: mixed activation types {t} and {o.dtype}")
+    return OGV_BF16 if t is torch.bfloat16 else OGV_F32
 
 
 def _device(what, first, *ts):
+    dev = first.device
     for t in (first, *ts):
-        if t is not None and not t.is_cuda:
-            raise RuntimeError(f"{what}: the MI355X kernels need HIP device tensors (got {t.device}); "
-                               f"this framework has no CPU execution path")
-        _need(t is None or t.device == first.device, f"{what}: tensors on {first.device} and {t.device if t is not None else None}")
+        if t is not None:
+            if not t.is_cuda:
+                raise RuntimeError(f"{what}: the MI355X kernels need HIP device tensors (got {t.device}); "
+                                   f"this framework has no CPU execution path")
+            if t.device != dev:
+                raise ValueError(f"{what}: tensors on {dev} and {t.device}")
 
 
-class _on:
-    """The tensors' device made current; yields its current stream's handle."""
+def _grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
-    def __init__(self, t):
-        self.guard = torch.cuda.device(t.device)
-        self.device = t.device
 
-    def __enter__(self):
-        self.guard.__enter__()
-        return _vp(torch.cuda.current_stream(self.device).cuda_stream)
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
-    def __exit__(self, *exc):
-        return self.guard.__exit__(*exc)
+
+def _launch(fn, name, like, *args):
+    """Call the C-ABI on the current stream of `like`'s device, with that device current."""
+    dev = like.device.index
+    if dev == torch.cuda.current_device():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)), name)
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)), name)
 
 
 def _ws(nbytes, like):
-    return torch.empty(int(nbytes), dtype=torch.uint8, device=like.device) if nbytes else None
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
 
 
 def _heads3(t):
     """A [rows, heads, D] tensor the kernels can address (unit last stride, 16-byte rows, heads and base), else a copy."""
     al = 16 // t.element_size()
-    if (t.shape[0] > 1 and t.stride(0) % al or t.shape[1] > 1 and t.stride(1) % al or t.stride(2) != 1 and t.shape[2] > 1
-            or t.data_ptr() % 16):
+    (m, h, d), (sm, sh, sd) = t.shape, t.stride()
+    if m > 1 and sm % al or h > 1 and sh % al or d > 1 and sd != 1 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _strides(t):
     """(row, head) strides; those of a size-1 dim are never used and may be anything in torch."""
-    return (t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
+    m, h, _ = t.shape
+    sm, sh, _ = t.stride()
+    return (sm if m > 1 else 0, sh if h > 1 else 0)
 
 
 # ------------------------------------------------------------------------------------------------
 # Attention
 # ------------------------------------------------------------------------------------------------
-def _packed_desc(B, q, k, v, causal, scale, **more):
-    d = PackedDesc(B=B, Mq=q.shape[0], Mk=k.shape[0], heads=q.shape[1], kv_heads=k.shape[1], D=q.shape[2],
-                   causal=int(causal), scale=scale)
-    for i, t in enumerate((q, k, v, more.get("out"), more.get("dout"), more.get("dq"), more.get("dk"), more.get("dv"))):
-        if t is not None:
-            d.row[i], d.head[i] = _strides(t)
-    return d
+@functools.lru_cache(4096)
+def _packed_desc(B, Mq, Mk, heads, kv_heads, D, causal, scale, dt, *strides):
+    """(descriptor, forward workspace bytes, backward workspace bytes)."""
+    d = PackedDesc(B=B, Mq=Mq, Mk=Mk, heads=heads, kv_heads=kv_heads, D=D, causal=causal, scale=scale)
+    for i, (row, head) in enumerate(strides):
+        d.row[i], d.head[i] = row, head
+    lib = _lib.load()
+    r = ctypes.byref(d)
+    return r, lib.ogv_packed_attn_fwd_ws_bytes(r, dt), lib.ogv_packed_attn_bwd_ws_bytes(r, dt)
 
 
 def _attn_fwd(q, k, v, cu_q, cu_k, causal, scale):
-    lib = _lib.load()
     dt = _dtype("ogv.packed_attention", q, k, v)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-    if q.shape[0] == 0:
+    Mq, heads, D = q.shape
+    out = torch.empty((Mq, heads, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((Mq, heads), dtype=torch.float32, device=q.device)
+    if Mq == 0:
         return out, lse
-    if cu_q.numel() == 1:   # no sequence at all: every row is behind the last one
+    B = cu_q.shape[0] - 1
+    if B == 0:   # no sequence at all: every row is behind the last one
         return out.zero_(), lse.fill_(-math.inf)
-    d = _packed_desc(cu_q.numel() - 1, q, k, v, causal, scale, out=out)
-    with _on(q) as stream:
-        ws = _ws(lib.ogv_packed_attn_fwd_ws_bytes(ctypes.byref(d), dt), q)
-        check(lib.ogv_packed_attn_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(cu_q), _ptr(cu_k), _ptr(out), _ptr(lse), _ptr(ws),
-                                      ctypes.byref(d), dt, stream), "ogv_packed_attn_fwd")
+    d, ws, _ = _packed_desc(B, Mq, k.shape[0], heads, k.shape[1], D, causal, scale, dt, _strides(q), _strides(k), _strides(v),
+                            (heads * D, D))
+    ws = _ws(ws, q)
+    _launch(_lib.load().ogv_packed_attn_fwd, "ogv_packed_attn_fwd", q, _ptr(q), _ptr(k), _ptr(v), _ptr(cu_q), _ptr(cu_k),
+            _ptr(out), _ptr(lse), _ptr(ws), d, dt)
     return out, lse
 
 
 def _attn_bwd(dout, q, k, v, out, lse, cu_q, cu_k, causal, scale, dq, dk, dv):
     """Writes dq, dk, dv (which may be strided)."""
-    lib = _lib.load()
     dt = _dtype("ogv.packed_attention", q, k, v, dout)
-    if q.shape[0] == 0 or cu_q.numel() == 1:
+    Mq, heads, D = q.shape
+    B = cu_q.shape[0] - 1
+    if Mq == 0 or B == 0:
         for t in (dq, dk, dv):
             t.zero_()
         return
-    d = _packed_desc(cu_q.numel() - 1, q, k, v, causal, scale, out=out, dout=dout, dq=dq, dk=dk, dv=dv)
-    with _on(q) as stream:
-        ws = _ws(lib.ogv_packed_attn_bwd_ws_bytes(ctypes.byref(d), dt), q)
-        check(lib.ogv_packed_attn_bwd(_ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(cu_q), _ptr(cu_k),
-                                      _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), ctypes.byref(d), dt, stream),
-              "ogv_packed_attn_bwd")
+    d, _, ws = _packed_desc(B, Mq, k.shape[0], heads, k.shape[1], D, causal, scale, dt,
+                            *(_strides(t) for t in (q, k, v, out, dout, dq, dk, dv)))
+    ws = _ws(ws, q)
+    _launch(_lib.load().ogv_packed_attn_bwd, "ogv_packed_attn_bwd", q, _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
+            _ptr(lse), _ptr(cu_q), _ptr(cu_k), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), d, dt)
 
 
 class _PackedAttention(torch.autograd.Function):
@@ -142,17 +154,20 @@ class _PackedAttention(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None
 
 
-def _check_cu(what, cu, like):
-    _need(cu.dtype == torch.int32 and cu.ndim == 1 and cu.numel() >= 1, f"{what}: int32 [sequences + 1] expected, got "
-          f"{cu.dtype} {tuple(cu.shape)}")
-    return cu.contiguous()
+def _check_cu(what, cu):
+    if cu.dtype is not torch.int32 or cu.ndim != 1 or cu.shape[0] < 1:
+        raise ValueError(f"{what}: int32 [sequences + 1] expected, got {cu.dtype} {tuple(cu.shape)}")
+    return cu if cu.is_contiguous() else cu.contiguous()
 
 
 def _check_attention(what, D, heads, kv_heads, scale):
-    _need(heads > 0 and kv_heads > 0 and heads % kv_heads == 0, f"{what}: heads ({heads}) must be a multiple of kv_heads ({kv_heads})")
-    _need(8 <= D <= 128 and D % 8 == 0, f"{what}: head_dim {D} unsupported (a multiple of 8 up to 128)")
+    if not (heads > 0 and kv_heads > 0 and heads % kv_heads == 0):
+        raise ValueError(f"{what}: heads ({heads}) must be a multiple of kv_heads ({kv_heads})")
+    if not (8 <= D <= 128 and D % 8 == 0):
+        raise ValueError(f"{what}: head_dim {D} unsupported (a multiple of 8 up to 128)")
     scale = D**-0.5 if scale is None else float(scale)
-    _need(0.0 < scale < math.inf, f"{what}: scale must be positive and finite, got {scale}")
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"{what}: scale must be positive and finite, got {scale}")
     return scale
 
 
@@ -168,51 +183,62 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal=False, scale=None, return_
     Returns out [rows, heads, D], with return_lse also the fp32 log-sum-exp [rows, heads] (no gradient).
     A non-finite value in v reaches its own sequence only, also where causal hides it."""
     what = "ogv.packed_attention"
-    _need(q.ndim == 3 and k.ndim == 3 and v.ndim == 3, f"{what}: q, k, v must be [rows, heads, head_dim]")
+    if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
+        raise ValueError(f"{what}: q, k, v must be [rows, heads, head_dim]")
     cu_k = cu_q if cu_k is None else cu_k
-    _need(k.shape == v.shape, f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
-    _need(q.shape[2] == k.shape[2], f"{what}: head_dim of q ({q.shape[2]}) and k ({k.shape[2]}) differ")
+    if k.shape != v.shape:
+        raise ValueError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+    if q.shape[2] != k.shape[2]:
+        raise ValueError(f"{what}: head_dim of q ({q.shape[2]}) and k ({k.shape[2]}) differ")
     scale = _check_attention(what, q.shape[2], q.shape[1], k.shape[1], scale)
     _dtype(what, q, k, v)
-    cu_q, cu_k = _check_cu(f"{what}: cu_q", cu_q, q), _check_cu(f"{what}: cu_k", cu_k, q)
-    _need(cu_q.numel() == cu_k.numel(), f"{what}: cu_q has {cu_q.numel()} offsets, cu_k {cu_k.numel()}")
+    cu_q, cu_k = _check_cu(f"{what}: cu_q", cu_q), _check_cu(f"{what}: cu_k", cu_k)
+    if cu_q.shape != cu_k.shape:
+        raise ValueError(f"{what}: cu_q has {cu_q.numel()} offsets, cu_k {cu_k.numel()}")
     _device(what, q, k, v, cu_q, cu_k)
-    out, lse = _PackedAttention.apply(_heads3(q), _heads3(k), _heads3(v), cu_q, cu_k, bool(causal), scale)
+    fn = _PackedAttention.apply if _grad(q, k, v) else _attn_fwd
+    out, lse = fn(_heads3(q), _heads3(k), _heads3(v), cu_q, cu_k, bool(causal), scale)
     return (out, lse) if return_lse else out
 
 
 # ------------------------------------------------------------------------------------------------
 # Rotary positions
 # ------------------------------------------------------------------------------------------------
+@functools.lru_cache(4096)
+def _rotary_desc(M, D, sections, theta, interleaved, inverse, pos_float, *tensors):
+    d = RotaryDesc(M=M, D=D, axes=len(sections), interleaved=interleaved, inverse=inverse, pos_float=pos_float, theta=theta)
+    for i, n in enumerate(sections):
+        d.pairs[i] = n
+    for i, (heads, a, b) in enumerate(tensors):
+        d.heads[i] = heads
+        (d.row_in[i], d.head_in[i]), (d.row_out[i], d.head_out[i]) = a, b
+    return ctypes.byref(d)
+
+
 def _rotate(xs, outs, positions, meta, inverse):
     """Turn the one or two [M, heads, D] tensors xs into outs."""
-    sections, theta, interleaved = meta
     x = xs[0]
     if x.shape[0] == 0:
         return
-    lib = _lib.load()
-    d = RotaryDesc(M=x.shape[0], D=x.shape[2], axes=len(sections), interleaved=int(interleaved), inverse=int(inverse),
-                   pos_float=int(positions.dtype == torch.float32), theta=theta)
-    for i, n in enumerate(sections):
-        d.pairs[i] = n
-    for i, (a, b) in enumerate(zip(xs, outs)):
-        d.heads[i] = a.shape[1]
-        d.row_in[i], d.head_in[i] = _strides(a)
-        d.row_out[i], d.head_out[i] = _strides(b)
+    d = _rotary_desc(x.shape[0], x.shape[2], *meta, inverse, positions.dtype is torch.float32,
+                     *((a.shape[1], _strides(a), _strides(b)) for a, b in zip(xs, outs)))
     k, k_out = (xs[1], outs[1]) if len(xs) > 1 else (None, None)
-    with _on(x) as stream:
-        check(lib.ogv_axial_rotary(_ptr(x), _ptr(outs[0]), _ptr(k), _ptr(k_out), _ptr(positions), ctypes.byref(d),
-                                   _dtype("ogv.axial_rotary", *xs), stream), "ogv_axial_rotary")
+    _launch(_lib.load().ogv_axial_rotary, "ogv_axial_rotary", x, _ptr(x), _ptr(outs[0]), _ptr(k), _ptr(k_out), _ptr(positions), d,
+            _dtype("ogv.axial_rotary", *xs))
+
+
+def _rotate_new(positions, meta, *xs):
+    outs = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)
+    _rotate(xs, outs, positions, meta, False)
+    return outs
 
 
 class _AxialRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, positions, meta, *xs):
-        outs = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)
-        _rotate(xs, outs, positions, meta, False)
         ctx.save_for_backward(positions)
         ctx.meta = meta
-        return outs
+        return _rotate_new(positions, meta, *xs)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -226,14 +252,19 @@ class _AxialRotary(torch.autograd.Function):
 
 def _check_rotary(what, D, positions, sections, theta, interleaved, rows):
     sections = tuple(int(n) for n in sections)
-    _need(1 <= len(sections) <= 4 and all(n > 0 for n in sections), f"{what}: sections must be 1 to 4 positive pair counts, got {sections}")
-    _need(D % 2 == 0 and D <= 128 and 2 * sum(sections) <= D, f"{what}: {sum(sections)} pairs need an even head_dim of at "
-          f"least {2 * sum(sections)} (and at most 128), got {D}")
-    _need(positions.dtype in (torch.int32, torch.float32), f"{what}: positions must be int32 or float32, got {positions.dtype}", TypeError)
-    _need(positions.shape == (rows, len(sections)), f"{what}: positions [rows, axes] = [{rows}, {len(sections)}] expected, got {tuple(positions.shape)}")
+    if not (1 <= len(sections) <= 4 and all(n > 0 for n in sections)):
+        raise ValueError(f"{what}: sections must be 1 to 4 positive pair counts, got {sections}")
+    if not (D % 2 == 0 and D <= 128 and 2 * sum(sections) <= D):
+        raise ValueError(f"{what}: {sum(sections)} pairs need an even head_dim of at "
+                         f"least {2 * sum(sections)} (and at most 128), got {D}")
+    if not (positions.dtype in (torch.int32, torch.float32)):
+        raise TypeError(f"{what}: positions must be int32 or float32, got {positions.dtype}")
+    if not (positions.shape == (rows, len(sections))):
+        raise ValueError(f"{what}: positions [rows, axes] = [{rows}, {len(sections)}] expected, got {tuple(positions.shape)}")
     theta = float(theta)
-    _need(0.0 < theta < math.inf, f"{what}: theta must be positive and finite, got {theta}")
-    return positions.detach().contiguous(), (sections, theta, bool(interleaved))
+    if not (0.0 < theta < math.inf):
+        raise ValueError(f"{what}: theta must be positive and finite, got {theta}")
+    return positions.detach() if positions.is_contiguous() else positions.detach().contiguous(), (sections, theta, bool(interleaved))
 
 
 def axial_rotary(q, k, positions, sections, theta=10000.0, interleaved=False):
@@ -245,15 +276,18 @@ def axial_rotary(q, k, positions, sections, theta=10000.0, interleaved=False):
     by position * theta^(-j / n); pair p is the dims (p, p + P), or (2p, 2p + 1) with interleaved; dims from 2 P
     on pass unchanged.  Angles are reduced in 64 bits.  Positions get no gradient."""
     what = "ogv.axial_rotary"
-    _need(q.ndim == 3 and (k is None or k.ndim == 3), f"{what}: q and k must be [rows, heads, head_dim]")
-    _need(q.shape[1] > 0 and (k is None or k.shape[1] > 0), f"{what}: no heads")
-    _need(k is None or (k.shape[0] == q.shape[0] and k.shape[2] == q.shape[2]),
-          f"{what}: q {tuple(q.shape)} and k {None if k is None else tuple(k.shape)} differ in rows or head_dim")
+    if not (q.ndim == 3 and (k is None or k.ndim == 3)):
+        raise ValueError(f"{what}: q and k must be [rows, heads, head_dim]")
+    if not (q.shape[1] > 0 and (k is None or k.shape[1] > 0)):
+        raise ValueError(f"{what}: no heads")
+    if not (k is None or (k.shape[0] == q.shape[0] and k.shape[2] == q.shape[2])):
+        raise ValueError(f"{what}: q {tuple(q.shape)} and k {None if k is None else tuple(k.shape)} differ in rows or head_dim")
     xs = (q,) if k is None else (q, k)
     _dtype(what, *xs)
     positions, meta = _check_rotary(what, q.shape[2], positions, sections, theta, interleaved, q.shape[0])
     _device(what, q, k, positions)
-    outs = _AxialRotary.apply(positions, meta, *(_heads3(x) for x in xs))
+    fn = _AxialRotary.apply if _grad(*xs) else _rotate_new
+    outs = fn(positions, meta, *(_heads3(x) for x in xs))
     return outs[0] if k is None else outs
 
 
@@ -299,14 +333,16 @@ def rotary_attention_rows(qkv, cu, heads, kv_heads=None, positions=None, section
     packed_attention(*axial_rotary(q, k, ...), v, cu), with one gradient buffer for all three."""
     what = "ogv.rotary_attention_rows"
     kv_heads = heads if kv_heads is None else int(kv_heads)
-    _need(qkv.ndim == 2, f"{what}: qkv must be [rows, columns]")
-    _need(heads > 0 and kv_heads > 0 and qkv.shape[1] % (heads + 2 * kv_heads) == 0,
-          f"{what}: {qkv.shape[1]} columns do not split into {heads} + 2 * {kv_heads} heads")
+    if not (qkv.ndim == 2):
+        raise ValueError(f"{what}: qkv must be [rows, columns]")
+    if not (heads > 0 and kv_heads > 0 and qkv.shape[1] % (heads + 2 * kv_heads) == 0):
+        raise ValueError(f"{what}: {qkv.shape[1]} columns do not split into {heads} + 2 * {kv_heads} heads")
     D = qkv.shape[1] // (heads + 2 * kv_heads)
     scale = _check_attention(what, D, heads, kv_heads, scale)
     _dtype(what, qkv)
-    cu = _check_cu(f"{what}: cu", cu, qkv)
-    _need((positions is None) == (sections is None), f"{what}: positions and sections belong together")
+    cu = _check_cu(f"{what}: cu", cu)
+    if not ((positions is None) == (sections is None)):
+        raise ValueError(f"{what}: positions and sections belong together")
     rot = None
     if positions is not None:
         positions, rot = _check_rotary(what, D, positions, sections, theta, interleaved, qkv.shape[0])
@@ -320,27 +356,33 @@ def rotary_attention_rows(qkv, cu, heads, kv_heads=None, positions=None, section
 # ------------------------------------------------------------------------------------------------
 # Norms around a gated residual
 # ------------------------------------------------------------------------------------------------
+@functools.lru_cache(4096)
+def _norm_desc(M, C, post, pre, samples, rps, alpha, post_eps, pre_eps, dt):
+    """(descriptor, backward workspace bytes)."""
+    d = ctypes.byref(GatedNormDesc(M=M, C=C, post=post, pre=pre, samples=samples, rps=rps, alpha=alpha, post_eps=post_eps,
+                                   pre_eps=pre_eps))
+    return d, _lib.load().ogv_gated_norm_bwd_ws_bytes(d, dt)
+
+
+def _norm_fwd(f, x, gate, rs, post_w, post_b, pre_w, pre_b, meta, stats=None):
+    dt = _dtype("ogv.gated_residual_norm", f, x)
+    y = torch.empty_like(f)
+    h = torch.empty_like(f) if meta[1] else None
+    if f.shape[0]:
+        _launch(_lib.load().ogv_gated_norm_fwd, "ogv_gated_norm_fwd", f, _ptr(f), _ptr(x), _ptr(gate), _ptr(rs), _ptr(post_w),
+                _ptr(post_b), _ptr(pre_w), _ptr(pre_b), _ptr(y), _ptr(h), _ptr(stats), _norm_desc(*f.shape, *meta, dt)[0], dt)
+    return y if h is None else (y, h)
+
+
 class _GatedNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, f, x, gate, rs, post_w, post_b, pre_w, pre_b, meta):
-        lib = _lib.load()
-        dt = _dtype("ogv.gated_residual_norm", f, x)
-        M, C = f.shape
-        post, pre, samples, rps, alpha, post_eps, pre_eps = meta
-        d = GatedNormDesc(M=M, C=C, post=post, pre=pre, samples=samples, rps=rps, alpha=alpha, post_eps=post_eps,
-                          pre_eps=pre_eps)
-        y = torch.empty_like(f)
-        h = torch.empty_like(f) if pre else None
-        stats = torch.empty((M, 4), dtype=torch.float32, device=f.device) if any(ctx.needs_input_grad) else None
-        if M:
-            with _on(f) as stream:
-                check(lib.ogv_gated_norm_fwd(_ptr(f), _ptr(x), _ptr(gate), _ptr(rs), _ptr(post_w), _ptr(post_b),
-                                             _ptr(pre_w), _ptr(pre_b), _ptr(y), _ptr(h), _ptr(stats), ctypes.byref(d), dt,
-                                             stream), "ogv_gated_norm_fwd")
+        stats = torch.empty((f.shape[0], 4), dtype=torch.float32, device=f.device)
+        out = _norm_fwd(f, x, gate, rs, post_w, post_b, pre_w, pre_b, meta, stats)
         ctx.save_for_backward(f, x, gate, rs, post_w, post_b, pre_w, pre_b, stats)
-        ctx.meta = d
+        ctx.meta = meta
         ctx.set_materialize_grads(False)
-        return (y, h) if pre else y
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -348,20 +390,18 @@ class _GatedNorm(torch.autograd.Function):
         f, x, gate, rs, post_w, post_b, pre_w, pre_b, stats = ctx.saved_tensors
         if dy is None and dh is None:
             return (None,) * 9
-        d, lib = ctx.meta, _lib.load()
         M, C = f.shape
         dy, dh = (None if g is None else g.to(f.dtype).contiguous() for g in (dy, dh))
         df, dx = torch.empty_like(f), torch.empty_like(f)
         sums = torch.empty((5, C), dtype=torch.float32, device=f.device)
-        dgate = torch.empty_like(gate) if d.samples > 1 and gate is not None else None
+        dgate = torch.empty_like(gate) if gate is not None and ctx.meta[2] > 1 else None
         if M:
-            with _on(f) as stream:
-                dt = _dtype("ogv.gated_residual_norm", f)
-                ws = _ws(lib.ogv_gated_norm_bwd_ws_bytes(ctypes.byref(d), dt), f)
-                check(lib.ogv_gated_norm_bwd(_ptr(dy), _ptr(dh), _ptr(f), _ptr(x), _ptr(gate), _ptr(rs), _ptr(post_w),
-                                             _ptr(post_b), _ptr(pre_w), _ptr(pre_b), _ptr(stats), _ptr(df), _ptr(dx),
-                                             _ptr(sums), _ptr(dgate), _ptr(ws), ctypes.byref(d), dt, stream),
-                      "ogv_gated_norm_bwd")
+            dt = _dtype("ogv.gated_residual_norm", f)
+            d, ws = _norm_desc(M, C, *ctx.meta, dt)
+            ws = _ws(ws, f)
+            _launch(_lib.load().ogv_gated_norm_bwd, "ogv_gated_norm_bwd", f, _ptr(dy), _ptr(dh), _ptr(f), _ptr(x), _ptr(gate),
+                    _ptr(rs), _ptr(post_w), _ptr(post_b), _ptr(pre_w), _ptr(pre_b), _ptr(stats), _ptr(df), _ptr(dx), _ptr(sums),
+                    _ptr(dgate), _ptr(ws), d, dt)
         else:
             sums.zero_()
             dgate = torch.zeros_like(gate) if dgate is not None else None
@@ -382,31 +422,42 @@ def gated_residual_norm(branch, residual, gate=None, row_scale=None, rps=1, alph
     each.  row_scale fp32, one factor per rps rows (DropPath's; it gets no gradient).
     Returns (y, h), or y alone without a pre_norm.  h comes from y before its rounding.  C <= 8192."""
     what = "ogv.gated_residual_norm"
-    _need(branch.ndim == 2 and branch.shape == residual.shape, f"{what}: branch {tuple(branch.shape)} and residual "
-          f"{tuple(residual.shape)} must be equal [rows, channels]")
+    if not (branch.ndim == 2 and branch.shape == residual.shape):
+        raise ValueError(f"{what}: branch {tuple(branch.shape)} and residual "
+                         f"{tuple(residual.shape)} must be equal [rows, channels]")
     M, C = branch.shape
-    _need(post_norm in NORMS and pre_norm in NORMS, f"{what}: norms are 'layer', 'rms' or None, got {post_norm!r}, {pre_norm!r}")
-    _need(1 <= C <= 8192, f"{what}: {C} channels unsupported (1 to 8192)")
+    if not (post_norm in NORMS and pre_norm in NORMS):
+        raise ValueError(f"{what}: norms are 'layer', 'rms' or None, got {post_norm!r}, {pre_norm!r}")
+    if not (1 <= C <= 8192):
+        raise ValueError(f"{what}: {C} channels unsupported (1 to 8192)")
     _dtype(what, branch, residual)
     post, pre = NORMS[post_norm], NORMS[pre_norm]
-    _need(post or (post_weight is None and post_bias is None), f"{what}: weights for an absent post_norm")
-    _need(pre or (pre_weight is None and pre_bias is None), f"{what}: weights for an absent pre_norm")
+    if not (post or (post_weight is None and post_bias is None)):
+        raise ValueError(f"{what}: weights for an absent post_norm")
+    if not (pre or (pre_weight is None and pre_bias is None)):
+        raise ValueError(f"{what}: weights for an absent pre_norm")
     params = []
     for name, p in (("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight), ("pre_bias", pre_bias)):
-        _need(p is None or p.shape == (C,), f"{what}: {name} must be [{C}]")
+        if not (p is None or p.shape == (C,)):
+            raise ValueError(f"{what}: {name} must be [{C}]")
         params.append(None if p is None else f32(p).contiguous())
     samples = 1
     if gate is not None:
-        _need(gate.ndim in (1, 2) and gate.shape[-1] == C, f"{what}: gate must be [{C}] or [samples, {C}], got {tuple(gate.shape)}")
+        if not (gate.ndim in (1, 2) and gate.shape[-1] == C):
+            raise ValueError(f"{what}: gate must be [{C}] or [samples, {C}], got {tuple(gate.shape)}")
         if gate.ndim == 2:
             samples = gate.shape[0]
-            _need(samples >= 1 and M % samples == 0, f"{what}: {M} rows do not divide into {samples} samples")
+            if not (samples >= 1 and M % samples == 0):
+                raise ValueError(f"{what}: {M} rows do not divide into {samples} samples")
         gate = f32(gate).contiguous()
     rps = int(rps)
-    _need(rps >= 1, f"{what}: rps must be >= 1")
+    if not (rps >= 1):
+        raise ValueError(f"{what}: rps must be >= 1")
     if row_scale is not None:
-        _need(row_scale.numel() * rps >= M, f"{what}: row_scale has {row_scale.numel()} factors of {rps} rows for {M} rows")
+        if not (row_scale.numel() * rps >= M):
+            raise ValueError(f"{what}: row_scale has {row_scale.numel()} factors of {rps} rows for {M} rows")
         row_scale = row_scale.detach().float().reshape(-1).contiguous()
     _device(what, branch, residual, gate, row_scale, *params)
     meta = (post, pre, samples, rps, float(alpha), float(post_eps), float(pre_eps))
-    return _GatedNorm.apply(branch.contiguous(), residual.contiguous(), gate, row_scale, *params, meta)
+    fn = _GatedNorm.apply if _grad(branch, residual, gate, *params) else _norm_fwd
+    return fn(branch.contiguous(), residual.contiguous(), gate, row_scale, *params, meta)

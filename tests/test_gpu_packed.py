@@ -125,7 +125,11 @@ def test_attention_layouts():
     # one key / value head broadcast to all: the gradient of the one is the sum over the copies
     k1, v1 = k[:, :1].clone().requires_grad_(), v[:, :1].clone().requires_grad_()
     out = packed_attention(q, k1.expand(-1, h, -1), v1.expand(-1, h, -1), cu, causal=True)
-    assert torch.equal(out, packed_attention(q, k1, v1, cu, causal=True))
+    # (as shared heads the rows are grouped into other tiles, of another size: each result is within its bound of the
+    # exact one, so they differ by two bounds at most)
+    tol = R.attention(q, k1, v1, lengths, lengths, True, D**-0.5, BF)["out"][1]
+    shared = packed_attention(q, k1, v1, cu, causal=True)
+    assert ((out.double() - shared.double()).abs().cpu() <= 2 * tol).all()
     a = torch.autograd.grad(out, (k1, v1), do)
     b = torch.autograd.grad(packed_attention(q, k1, v1, cu, causal=True), (k1, v1), do)
     for x, y in zip(a, b):   # h rounded gradients added (3 roundings of the sum too) against one rounding
