@@ -26,15 +26,42 @@ namespace ogv {
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((address_space(3))) s16x4 lds_tr_t;
 
+// Workgroup -> (key / value head, tile slot).  Each head is dealt to as few XCDs as an even share allows, tile slots
+// alternating between them: the workgroups of an XCD walk the same keys (its L2 holds them) and every XCD gets
+// the same mix of early and late tiles, which differ in work under the causal mask.
+struct Deal {
+  int parts;   // interleaved parts of a head
+  int per;     // tile slots of a part
+};
+static inline Deal deal(int hkv, int tiles) {
+  int g = 8;
+  while (hkv % g) g >>= 1;
+  const int parts = 8 / g;
+  return Deal{parts, (tiles + parts - 1) / parts};
+}
+static inline unsigned deal_grid(int hkv, int tiles) {
+  const Deal d = deal(hkv, tiles);
+  return (unsigned)((long)hkv * d.parts * d.per);
+}
+__device__ __forceinline__ bool head_tile(const Deal d, int hkv, int tiles, int& h, int& t) {
+  const int x = blockIdx.x & 7, y = blockIdx.x >> 3, mine = hkv * d.parts / 8;
+  const int part = x * mine + y / d.per;
+  h = part / d.parts;
+  t = (y % d.per) * d.parts + part % d.parts;
+  return t < tiles;
+}
+
 struct PackedArgs {
   const void *q, *k, *v, *o, *dout;   // o: forward's output (read by the backward)
   void *out, *dq, *dk, *dv;
   float *lse, *delta;
   const int *cu_q, *cu_k;
-  float *part_o, *part_ml;            // split forward: [split][Mq * hq][D] and [split][Mq * hq][2]
+  float *part_o, *part_ml;            // split forward: [piece][Mq * hq][D] and [piece][Mq * hq][2]
+  int* part_n;                        // split forward: pieces of a row
   int B, Mq, Mk, hq, hkv, D, G, causal;
   unsigned gmagic;                    // ceil(2^32 / G); r / G = umulhi(r, gmagic) for r * G < 2^32
-  int tiles, nsplit;                  // tile slots per key / value head; key splits
+  Deal d;                             // workgroups of the unsplit kernels
+  int tiles, nsplit, chunk;           // tile slots per key / value head; most key pieces of a row, fewest keys of a piece
   float scale;
   long rq, rk, rv, ro, rdo, rdq, rdk, rdv;   // row strides, elements
   long hsq, hsk, hsv, hso, hsdo, hsdq, hsdk, hsdv;   // head strides, elements
@@ -201,6 +228,49 @@ __device__ __forceinline__ Seq find_tile(const int* __restrict__ cu, int B, int 
   s.len = __builtin_amdgcn_readfirstlane(max(cu_at(cu, s.b + 1, M) - s.start, 0));
   s.tile = t - ((int)(((long)s.start * G) / BM) + s.b);
   return s;
+}
+
+// Key pieces of a sequence in the split forward: whole 64-key tiles, at least `chunk` keys, at most `most` pieces.
+__device__ __forceinline__ int piece_keys(int lk, int chunk, int most) {
+  return max(chunk, ((lk + most - 1) / most + 63) & ~63);
+}
+
+// Work item t of the split forward = (sequence, row tile, key piece), sequences in order, a sequence's pieces of
+// one row tile next to each other.  Returns false past the last item.  The whole wave searches, 64 sequences at a time.
+struct Piece {
+  int b, tile, piece;
+};
+__device__ __forceinline__ bool find_piece(const PackedArgs& a, int BM, int t, int lane, Piece& p) {
+  int base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + lane;
+    int n = 0, pieces = 1;
+    if (b < a.B) {
+      const int q0 = cu_at(a.cu_q, b, a.Mq), k0 = cu_at(a.cu_k, b, a.Mk);
+      const int lq = max((b == a.B - 1 ? a.Mq : cu_at(a.cu_q, b + 1, a.Mq)) - q0, 0);   // the last one's rows and those behind
+      const int lk = max(cu_at(a.cu_k, b + 1, a.Mk) - k0, 0);
+      const int keys = piece_keys(lk, a.chunk, a.nsplit);
+      pieces = max(1, (lk + keys - 1) / keys);
+      n = (int)(((long)lq * a.G + BM - 1) / BM) * pieces;
+    }
+    int sum = n;   // inclusive sum over the lanes
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += v;
+    }
+    const unsigned long long over = __ballot(base + sum > t);
+    if (over) {
+      const int w = __builtin_ctzll(over);
+      const int item = t - (base + __shfl(sum - n, w, 64)), pw = __shfl(pieces, w, 64);
+      p.b = __builtin_amdgcn_readfirstlane(b0 + w);
+      p.tile = __builtin_amdgcn_readfirstlane(item / pw);
+      p.piece = __builtin_amdgcn_readfirstlane(item % pw);
+      return true;
+    }
+    base += __shfl(sum, 63, 64);
+  }
+  return false;
 }
 
 }  // namespace ogv

@@ -29,10 +29,9 @@ __global__ __launch_bounds__(NW * 64) void packed_dq_kernel(const PackedArgs a) 
   __shared__ __attribute__((aligned(16))) char Vs[BN * RB];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hf = lane >> 5, c = lane & 31;
 
-  long id;
-  if (!xcd_block((long)a.hkv * a.tiles, id)) return;
-  const int h = (int)(id / a.tiles), t = a.tiles - 1 - (int)(id % a.tiles);
-  const Seq sq = find_tile(a.cu_q, a.B, a.Mq, a.G, BM, t, lane);
+  int h, t;
+  if (!head_tile(a.d, a.hkv, a.tiles, h, t)) return;
+  const Seq sq = find_tile(a.cu_q, a.B, a.Mq, a.G, BM, a.tiles - 1 - t, lane);
   const int k0 = cu_at(a.cu_k, sq.b, a.Mk), lk = max(cu_at(a.cu_k, sq.b + 1, a.Mk) - k0, 0);
   const int rows = sq.len * a.G, r0 = sq.tile * BM;
   const int store_rows = sq.b == a.B - 1 ? (a.Mq - sq.start) * a.G : rows;
@@ -142,9 +141,8 @@ __global__ __launch_bounds__(NW * 64) void packed_dkv_kernel(const PackedArgs a)
   __shared__ __attribute__((aligned(16))) int Lim[BN];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hf = lane >> 5, c = lane & 31;
 
-  long id;
-  if (!xcd_block((long)a.hkv * a.tiles, id)) return;
-  const int h = (int)(id / a.tiles), t = (int)(id % a.tiles);
+  int h, t;
+  if (!head_tile(a.d, a.hkv, a.tiles, h, t)) return;
   const Seq sk = find_tile(a.cu_k, a.B, a.Mk, 1, BM, t, lane);
   const int q0 = cu_at(a.cu_q, sk.b, a.Mq), lq = max(cu_at(a.cu_q, sk.b + 1, a.Mq) - q0, 0);
   const int j0 = sk.tile * BM, off = sk.len - lq, rows = lq * a.G;
@@ -257,12 +255,14 @@ static void bwd_launch(PackedArgs a, hipStream_t s) {
   const long rows = (long)a.Mq * a.G;
   const int nwq = rows >= 96L * a.B ? 4 : 1, nwk = a.Mk >= 96L * a.B ? 4 : 1;
   a.tiles = (int)(rows / (32 * nwq)) + a.B;
-  const unsigned nq = xcd_grid((long)a.hkv * a.tiles);
+  a.d = deal(a.hkv, a.tiles);
+  const unsigned nq = deal_grid(a.hkv, a.tiles);
   if (nwq == 4) packed_dq_kernel<T, D, 4><<<nq, 256, 0, s>>>(a);
   else packed_dq_kernel<T, D, 1><<<nq, 64, 0, s>>>(a);
   if (a.Mk == 0) return;
   a.tiles = a.Mk / (32 * nwk) + a.B;
-  const unsigned nk = xcd_grid((long)a.hkv * a.tiles);
+  a.d = deal(a.hkv, a.tiles);
+  const unsigned nk = deal_grid(a.hkv, a.tiles);
   if (nwk == 4) packed_dkv_kernel<T, D, 4><<<nk, 256, 0, s>>>(a);
   else packed_dkv_kernel<T, D, 1><<<nk, 64, 0, s>>>(a);
 }

@@ -82,34 +82,30 @@ __device__ __forceinline__ void fwd_tile(const char* Ks, const char* Vs, const C
   for (int nb = 0; nb < NB; ++nb) accum_xt<T, D>(Vs, nb * 32, s[nb], o, lane);
 }
 
+// One row tile over keys kt0 * BN .. of its sequence.
 template <typename T, int D, int NW, bool SPLIT>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_fwd_kernel(const PackedArgs a) {
+__device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* K0, char* V0, char* K1, char* V1, int h, int b, int tile, int piece) {
   using F = Frag<T, D>;
   constexpr int BM = 32 * NW, BN = sizeof(T) == 2 && NW > 1 ? 64 : 32, NB = BN / 32;
-  constexpr int RB = F::RB, KK = F::KK, E = F::E;
-  __shared__ __attribute__((aligned(16))) char K0[BN * RB], V0[BN * RB], K1[BN * RB], V1[BN * RB];
+  constexpr int KK = F::KK, E = F::E;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5, c = lane & 31;
-
-  long id;
-  if (!xcd_block((long)a.hkv * a.tiles * a.nsplit, id)) return;
-  const int split = SPLIT ? (int)(id % a.nsplit) : 0;
-  const long ht = SPLIT ? id / a.nsplit : id;
-  const int h = (int)(ht / a.tiles), t = a.tiles - 1 - (int)(ht % a.tiles);
-  const Seq sq = find_tile(a.cu_q, a.B, a.Mq, a.G, BM, t, lane);
-  const int k0 = __builtin_amdgcn_readfirstlane(cu_at(a.cu_k, sq.b, a.Mk));
-  const int lk = __builtin_amdgcn_readfirstlane(max(cu_at(a.cu_k, sq.b + 1, a.Mk) - k0, 0));
-  const int rows = sq.len * a.G, r0 = sq.tile * BM;
+  const int start = __builtin_amdgcn_readfirstlane(cu_at(a.cu_q, b, a.Mq));
+  const int len = __builtin_amdgcn_readfirstlane(max(cu_at(a.cu_q, b + 1, a.Mq) - start, 0));
+  const int k0 = __builtin_amdgcn_readfirstlane(cu_at(a.cu_k, b, a.Mk));
+  const int lk = __builtin_amdgcn_readfirstlane(max(cu_at(a.cu_k, b + 1, a.Mk) - k0, 0));
+  const int rows = len * a.G, r0 = tile * BM;
   // rows behind the last sequence belong to nothing: zeros
-  const int store_rows = sq.b == a.B - 1 ? (a.Mq - sq.start) * a.G : rows;
+  const int store_rows = b == a.B - 1 ? (a.Mq - start) * a.G : rows;
   if (r0 >= store_rows) return;
-  const int off = lk - sq.len;
+  const int off = lk - len;
   int kend = r0 < rows ? lk : 0;
   if (a.causal && kend) kend = max(0, min(lk, group_div(min(r0 + BM, rows) - 1, a.G, a.gmagic) + off + 1));
-  int kt0 = 0, kt1 = (kend + BN - 1) / BN;
+  int kt0 = 0, kt1 = (kend + BN - 1) / BN, pieces = 1;
   if (SPLIT) {
-    const int per = (kt1 + a.nsplit - 1) / a.nsplit;
-    kt0 = min(split * per, kt1);
-    kt1 = min(kt0 + per, kt1);
+    const int keys = piece_keys(lk, a.chunk, a.nsplit);
+    pieces = max(1, (lk + keys - 1) / keys);
+    kt0 = min(piece * (keys / BN), kt1);
+    kt1 = min(kt0 + keys / BN, kt1);
   }
 
   const T* kb = (const T*)a.k + (long)k0 * a.rk + (long)h * a.hsk;
@@ -128,7 +124,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_fwd_ke
   const int lim = live ? (a.causal ? min(lk - 1, pos + off) : lk - 1) : -1;   // last visible key
   Chunk qf[KK];
   {
-    const T* qp = (const T*)a.q + (long)(sq.start + (live ? pos : 0)) * a.rq + (long)(h * a.G + hg) * a.hsq;
+    const T* qp = (const T*)a.q + (long)(start + (live ? pos : 0)) * a.rq + (long)(h * a.G + hg) * a.hsq;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       const int d = (2 * kk + hf) * E;
@@ -155,9 +151,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_fwd_ke
 
   l += __shfl_xor(l, 32, 64);
   if (r >= store_rows) return;
-  const long orow = (long)(sq.start + pos) * a.hq + h * a.G + hg;   // row of the [Mq * hq] outputs
+  const long orow = (long)(start + pos) * a.hq + h * a.G + hg;   // row of the [Mq * hq] outputs
   if (SPLIT) {   // unnormalised partials, joined by packed_join_kernel
-    float* po = a.part_o + ((long)split * a.Mq * a.hq + orow) * a.D;
+    const long at = (long)piece * a.Mq * a.hq + orow;
+    float* po = a.part_o + at * a.D;
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
@@ -166,14 +163,13 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_fwd_ke
         if (d < a.D) *reinterpret_cast<float4*>(po + d) = make_float4(o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]);
       }
     if (hf == 0) {
-      float* ml = a.part_ml + 2 * ((long)split * a.Mq * a.hq + orow);
-      ml[0] = m;
-      ml[1] = l;
+      *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(m, l);
+      if (piece == 0) a.part_n[orow] = pieces;
     }
     return;
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);   // (NaN stays NaN)
-  T* op = (T*)a.out + (long)(sq.start + pos) * a.ro + (long)(h * a.G + hg) * a.hso;
+  T* op = (T*)a.out + (long)(start + pos) * a.ro + (long)(h * a.G + hg) * a.hso;
 #pragma unroll
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
@@ -187,23 +183,44 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_fwd_ke
   if (hf == 0) a.lse[orow] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
 }
 
-// out = sum_s w_s o_s / sum_s w_s l_s, w_s = exp(scale (m_s - max m)), over the key splits, in split order
+template <typename T, int D, int NW, bool SPLIT>
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_fwd_kernel(const PackedArgs a) {
+  constexpr int TB = (sizeof(T) == 2 && NW > 1 ? 64 : 32) * Frag<T, D>::RB;
+  __shared__ __attribute__((aligned(16))) char K0[TB], V0[TB], K1[TB], V1[TB];
+  const int lane = threadIdx.x & 63;
+  if (SPLIT) {   // every piece of work, head by head
+    for (int n = blockIdx.x;; n += gridDim.x) {
+      Piece p;
+      if (!find_piece(a, 32 * NW, n / a.hkv, lane, p)) return;
+      fwd_rows<T, D, NW, true>(a, K0, V0, K1, V1, n % a.hkv, p.b, p.tile, p.piece);
+      __syncthreads();   // the tiles are free again
+    }
+  } else {
+    int h, t;
+    if (!head_tile(a.d, a.hkv, a.tiles, h, t)) return;
+    const Seq sq = find_tile(a.cu_q, a.B, a.Mq, a.G, 32 * NW, a.tiles - 1 - t, lane);
+    fwd_rows<T, D, NW, false>(a, K0, V0, K1, V1, h, sq.b, sq.tile, 0);
+  }
+}
+
+// out = sum_s w_s o_s / sum_s w_s l_s, w_s = exp(scale (m_s - max m)), over a row's key pieces in order
 template <typename T>
 __global__ __launch_bounds__(256) void packed_join_kernel(const PackedArgs a) {
   const int per = a.D / 4;
   const long n = (long)a.Mq * a.hq * per, idx = (long)blockIdx.x * 256 + threadIdx.x;
   if (idx >= n) return;
   const long row = idx / per, R = (long)a.Mq * a.hq;
-  const int d = (int)(idx - row * per) * 4;
+  const int d = (int)(idx - row * per) * 4, pieces = a.part_n[row];
   float m = -INFINITY;
-  for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, a.part_ml[2 * (s * R + row)]);
-  const float mu = m == -INFINITY ? 0.f : m;
-  const float c2 = a.scale * LOG2E;
+  for (int s = 0; s < pieces; ++s) m = fmaxf(m, a.part_ml[2 * (s * R + row)]);
+  const float mu = m == -INFINITY ? 0.f : m, c2 = a.scale * LOG2E;
   float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.nsplit; ++s) {
-    const float w = __builtin_amdgcn_exp2f((a.part_ml[2 * (s * R + row)] - mu) * c2);
-    l += w * a.part_ml[2 * (s * R + row) + 1];
+#pragma unroll 4
+  for (int s = 0; s < pieces; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (s * R + row));
     const float4 p = *reinterpret_cast<const float4*>(a.part_o + (s * R + row) * a.D + d);
+    const float w = __builtin_amdgcn_exp2f((ml.x - mu) * c2);
+    l += w * ml.y;
     x[0] += w * p.x, x[1] += w * p.y, x[2] += w * p.z, x[3] += w * p.w;
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
@@ -215,34 +232,39 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const PackedArgs a) {
 }
 
 struct FwdPlan {
-  int nw, tiles, nsplit;
+  int nw, tiles, nsplit, chunk;
+  unsigned grid;
 };
 
-// Shortest sequences that fill four waves' rows on average get them, others one wave per workgroup;
-// the keys are split while the workgroups would not fill the 256 CUs.
+// Sequences that fill four waves' rows on average get them, others one wave per workgroup.  While the row tiles
+// would not fill the 256 CUs twice, the keys are split into pieces of equal size (not equal number: sequences
+// differ), about 1024 in all.
 static FwdPlan fwd_plan(const ogv_packed_desc* d) {
   FwdPlan p;
   const long rows = (long)d->Mq * (d->heads / d->kv_heads);
   p.nw = rows >= 96L * d->B ? 4 : 1;
   p.tiles = (int)(rows / (32 * p.nw)) + d->B;
-  const long blocks = (long)p.tiles * d->kv_heads, keys = d->Mk / d->B;
-  long n = blocks >= 512 ? 1 : 1024 / (blocks > 0 ? blocks : 1);
-  const long most = keys / 256;   // at least 256 keys to a split
-  if (n > most) n = most;
-  p.nsplit = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+  const long blocks = (long)p.tiles * d->kv_heads;
+  long chunk = ((long)d->Mk * blocks / d->B / 1024 + 63) & ~63L;   // keys read by all row tiles over 1024
+  if (chunk < 128) chunk = 128;
+  p.chunk = (int)(chunk < (1 << 30) ? chunk : 1 << 30);
+  const bool split = blocks < 512 && d->Mk / d->B >= 2 * chunk;
+  const long most = 4096 / (blocks > 0 ? blocks : 1);   // four times the average: bounds the workspace
+  p.nsplit = !split ? 1 : (int)(most < 2 ? 2 : most > 64 ? 64 : most);
+  long grid = blocks + (long)d->Mk / p.chunk * d->kv_heads * (p.tiles + d->B - 1) / d->B;
+  p.grid = split ? (unsigned)(grid < 4096 ? grid : 4096) : deal_grid(d->kv_heads, p.tiles);
   return p;
 }
 
 template <typename T, int D>
 static void fwd_launch(const FwdPlan& p, const PackedArgs& a, hipStream_t s) {
-  const unsigned nb = xcd_grid((long)a.hkv * p.tiles * p.nsplit);
   if (p.nsplit > 1) {
-    if (p.nw == 4) packed_fwd_kernel<T, D, 4, true><<<nb, 256, 0, s>>>(a);
-    else packed_fwd_kernel<T, D, 1, true><<<nb, 64, 0, s>>>(a);
+    if (p.nw == 4) packed_fwd_kernel<T, D, 4, true><<<p.grid, 256, 0, s>>>(a);
+    else packed_fwd_kernel<T, D, 1, true><<<p.grid, 64, 0, s>>>(a);
     packed_join_kernel<T><<<cdiv((long)a.Mq * a.hq * (a.D / 4), 256), 256, 0, s>>>(a);
   } else {
-    if (p.nw == 4) packed_fwd_kernel<T, D, 4, false><<<nb, 256, 0, s>>>(a);
-    else packed_fwd_kernel<T, D, 1, false><<<nb, 64, 0, s>>>(a);
+    if (p.nw == 4) packed_fwd_kernel<T, D, 4, false><<<p.grid, 256, 0, s>>>(a);
+    else packed_fwd_kernel<T, D, 1, false><<<p.grid, 64, 0, s>>>(a);
   }
 }
 
@@ -294,7 +316,7 @@ using namespace ogv;
 extern "C" size_t ogv_packed_attn_fwd_ws_bytes(const ogv_packed_desc* d, ogv_dtype dt) {
   if (packed_check("ogv_packed_attn_fwd_ws_bytes", d, dt) != OGV_OK) return 0;
   const FwdPlan p = fwd_plan(d);
-  return p.nsplit == 1 ? 0 : (size_t)p.nsplit * d->Mq * d->heads * (d->D + 2) * sizeof(float);
+  return p.nsplit == 1 ? 0 : ((size_t)p.nsplit * (d->D + 2) + 1) * d->Mq * d->heads * sizeof(float);
 }
 
 extern "C" int ogv_packed_attn_fwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k,
@@ -308,9 +330,11 @@ extern "C" int ogv_packed_attn_fwd(const void* q, const void* k, const void* v, 
   PackedArgs a;
   packed_args(d, a);
   a.q = q, a.k = k, a.v = v, a.cu_q = cu_q, a.cu_k = cu_k, a.out = out, a.lse = lse;
-  a.tiles = p.tiles, a.nsplit = p.nsplit;
+  a.d = deal(d->kv_heads, p.tiles), a.tiles = p.tiles, a.nsplit = p.nsplit, a.chunk = p.chunk;
+  const size_t n = (size_t)p.nsplit * d->Mq * d->heads;
   a.part_o = (float*)ws;
-  a.part_ml = (float*)ws + (size_t)p.nsplit * d->Mq * d->heads * d->D;
+  a.part_ml = (float*)ws + n * d->D;
+  a.part_n = (int*)((float*)ws + n * (d->D + 2));
   hipStream_t s = as_stream(stream);
 #define OGV_FWD(T)                                      \
   if (d->D <= 32) fwd_launch<T, 32>(p, a, s);           \
