@@ -54,7 +54,8 @@ __device__ __forceinline__ bool head_tile(const Deal d, int hkv, int tiles, int&
 struct PackedArgs {
   const void *q, *k, *v, *o, *dout;   // o: forward's output (read by the backward)
   void *out, *dq, *dk, *dv;
-  float *lse, *delta;
+  float* lse;
+  float2* rowstat;                    // backward: lse * log2(e) (+inf where no key is seen) and delta of a row
   const int *cu_q, *cu_k;
   float *part_o, *part_ml;            // split forward: [piece][Mq * hq][D] and [piece][Mq * hq][2]
   int* part_n;                        // split forward: pieces of a row

@@ -20,25 +20,79 @@ bool aligned16(std::initializer_list<const void*> ps);
 
 constexpr float BLOG2E = 1.4426950408889634f;
 
+// Store a 32-column C tile block (columns c, dims 32 * db + rows) times mul as rows of the output.
+template <typename T, int D>
+__device__ __forceinline__ void store_cols(T* p, const f32x16 (&x)[D / 32], float mul, int Dlive, int hf) {
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = db * 32 + 8 * g + 4 * hf;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = x[db][4 * g + e] * mul;
+      if (d < Dlive) store_vec<T, 4>(p + d, v);
+    }
+}
+
+// 32 * NB keys of dq: scores and dp transposed (columns are rows r), dQ^T += K^T dS^T
+template <typename T, int D, int NB>
+__device__ __forceinline__ void dq_tile(const char* Ks, const char* Vs, const Chunk (&qf)[Frag<T, D>::KK],
+                                        const Chunk (&gf)[Frag<T, D>::KK], f32x16 (&dq)[D / 32], int key0, int lim, float c2,
+                                        float lse2, float delta, int lane) {
+  constexpr int KK = Frag<T, D>::KK, RB = Frag<T, D>::RB;
+  const int hf = lane >> 5, c = lane & 31;
+#pragma unroll 1
+  for (int nb = 0; nb < NB; ++nb) {
+    f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      mfma_step<T>(lds_chunk<RB>(Ks, nb * 32 + c, 2 * kk + hf), qf[kk], s);
+      mfma_step<T>(lds_chunk<RB>(Vs, nb * 32 + c, 2 * kk + hf), gf[kk], dp);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -lse2)) * (dp[i] - delta);
+    if (!__all(key0 + nb * 32 + 31 <= lim)) {
+      rare_branch();
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (key0 + nb * 32 + 8 * (i / 4) + 4 * hf + i % 4 > lim) s[i] = 0.f;
+    }
+    accum_xt<T, D>(Ks, nb * 32, s, dq, lane);
+  }
+}
+
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64) void packed_dq_kernel(const PackedArgs a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dq_kernel(const PackedArgs a) {
   using F = Frag<T, D>;
-  constexpr int BM = 32 * NW, BN = 32, NT = NW * 64;
-  constexpr int RB = F::RB, NC = F::NC, KK = F::KK, E = F::E;
-  __shared__ __attribute__((aligned(16))) char Ks[BN * RB];
-  __shared__ __attribute__((aligned(16))) char Vs[BN * RB];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hf = lane >> 5, c = lane & 31;
+  constexpr int BM = 32 * NW, BN = sizeof(T) == 2 && NW > 1 ? 64 : 32, NB = BN / 32;
+  constexpr int RB = F::RB, KK = F::KK, E = F::E;
+  __shared__ __attribute__((aligned(16))) char K0[BN * RB], V0[BN * RB], K1[BN * RB], V1[BN * RB];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5, c = lane & 31;
 
   int h, t;
   if (!head_tile(a.d, a.hkv, a.tiles, h, t)) return;
   const Seq sq = find_tile(a.cu_q, a.B, a.Mq, a.G, BM, a.tiles - 1 - t, lane);
-  const int k0 = cu_at(a.cu_k, sq.b, a.Mk), lk = max(cu_at(a.cu_k, sq.b + 1, a.Mk) - k0, 0);
+  const int k0 = __builtin_amdgcn_readfirstlane(cu_at(a.cu_k, sq.b, a.Mk));
+  const int lk = __builtin_amdgcn_readfirstlane(max(cu_at(a.cu_k, sq.b + 1, a.Mk) - k0, 0));
   const int rows = sq.len * a.G, r0 = sq.tile * BM;
   const int store_rows = sq.b == a.B - 1 ? (a.Mq - sq.start) * a.G : rows;
   if (r0 >= store_rows) return;
   const int off = lk - sq.len;
   int kend = r0 < rows ? lk : 0;
   if (a.causal && kend) kend = max(0, min(lk, group_div(min(r0 + BM, rows) - 1, a.G, a.gmagic) + off + 1));
+  const int kt1 = (kend + BN - 1) / BN;
+
+  const T* kb = (const T*)a.k + (long)k0 * a.rk + (long)h * a.hsk;
+  const T* vb = (const T*)a.v + (long)k0 * a.rv + (long)h * a.hsv;
+  TileCopy<T, D, BN, NW> kc, vc;
+  kc.init(wave, lane, a.D, a.rk);
+  vc.init(wave, lane, a.D, a.rv);
+  auto stage = [&](int kt, char* Ks, char* Vs) {
+    kc.load(kb + (long)kt * BN * a.rk, a.rk, lk - kt * BN, Ks, wave, lane, a.D);
+    vc.load(vb + (long)kt * BN * a.rv, a.rv, lk - kt * BN, Vs, wave, lane, a.D);
+  };
+  if (kt1 > 0) stage(0, K0, V0);
 
   const int r = r0 + wave * 32 + c, pos = group_div(r, a.G, a.gmagic), hg = r - pos * a.G;
   const bool live = r < rows;
@@ -71,87 +125,113 @@ __global__ __launch_bounds__(NW * 64) void packed_dq_kernel(const PackedArgs a) 
     }
   }
   delta += __shfl_xor(delta, 32, 64);
-  if (live && hf == 0) a.delta[orow] = delta;
-  // a row that sees nothing has lse = -inf: its weights are masked below, +inf keeps the others' at 0
+  // a row that sees nothing has lse = -inf: +inf keeps its weights at exp2(-inf) = 0
   float lse2 = live ? a.lse[orow] * BLOG2E : INFINITY;
   if (lse2 == -INFINITY) lse2 = INFINITY;
+  if (live && hf == 0) a.rowstat[orow] = make_float2(lse2, delta);   // for the dk / dv kernel
   f32x16 dq[D / 32];
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) dq[db] = f32x16{};
   const float c2 = a.scale * BLOG2E;
-  const T* kb = (const T*)a.k + (long)k0 * a.rk + (long)h * a.hsk;
-  const T* vb = (const T*)a.v + (long)k0 * a.rv + (long)h * a.hsv;
 
-  for (int key0 = 0; key0 < kend; key0 += BN) {
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < (BN * NC + NT - 1) / NT; ++n) {
-      const int idx = tid + n * NT;
-      if (BN * NC % NT == 0 || idx < BN * NC) {
-        const int row = idx / NC, ch = idx - row * NC;
-        Chunk kc = zero_chunk(), vc = zero_chunk();
-        if (key0 + row < lk && ch * E < a.D) {
-          kc.u = *reinterpret_cast<const uint4*>(kb + (long)(key0 + row) * a.rk + ch * E);
-          vc.u = *reinterpret_cast<const uint4*>(vb + (long)(key0 + row) * a.rv + ch * E);
-        }
-        const int at = row * RB + ((ch ^ swz<RB>(row)) << 4);
-        *reinterpret_cast<uint4*>(Ks + at) = kc.u;
-        *reinterpret_cast<uint4*>(Vs + at) = vc.u;
-      }
-    }
-    __syncthreads();
-    f32x16 s = f32x16{}, dp = f32x16{};
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      mfma_step<T>(lds_chunk<RB>(Ks, c, 2 * kk + hf), qf[kk], s);
-      mfma_step<T>(lds_chunk<RB>(Vs, c, 2 * kk + hf), gf[kk], dp);
-    }
-    const bool masked = !__all(key0 + BN - 1 <= lim);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float p = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -lse2)) * (dp[i] - delta);
-      if (masked && key0 + 8 * (i / 4) + 4 * hf + i % 4 > lim) p = 0.f;
-      s[i] = p;
-    }
-    accum_xt<T, D>(Ks, 0, s, dq, lane);
+  for (int kt = 0; kt < kt1; kt += 2) {
+    tiles_ready();
+    if (kt + 1 < kt1) stage(kt + 1, K1, V1);
+    dq_tile<T, D, NB>(K0, V0, qf, gf, dq, kt * BN, lim, c2, lse2, delta, lane);
+    if (kt + 1 >= kt1) break;
+    tiles_ready();
+    if (kt + 2 < kt1) stage(kt + 2, K0, V0);
+    dq_tile<T, D, NB>(K1, V1, qf, gf, dq, (kt + 1) * BN, lim, c2, lse2, delta, lane);
   }
 
   if (r >= store_rows) return;
-  T* qp = (T*)a.dq + (long)(sq.start + pos) * a.rdq + (long)(h * a.G + hg) * a.hsdq;
+  store_cols<T, D>((T*)a.dq + (long)(sq.start + pos) * a.rdq + (long)(h * a.G + hg) * a.hsdq, dq, a.scale, a.D, hf);
+}
+
+// 32 * NB rows of dk / dv: scores and dp with columns = keys, dV^T += dO^T P, dK^T += Q^T dS
+template <typename T, int D, int NB>
+__device__ __forceinline__ void dkv_tile(const char* Qs, const char* Gs, const float2* St, const Chunk (&kf)[Frag<T, D>::KK],
+                                         const Chunk (&vf)[Frag<T, D>::KK], f32x16 (&dk)[D / 32], f32x16 (&dv)[D / 32], int rt,
+                                         int off, int j, int jmax, const PackedArgs& a, float c2, int lane) {
+  constexpr int KK = Frag<T, D>::KK, RB = Frag<T, D>::RB;
+  const int hf = lane >> 5, c = lane & 31;
+#pragma unroll 1
+  for (int nb = 0; nb < NB; ++nb) {
+    f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
-  for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = db * 32 + 8 * g + 4 * hf;
-      float x[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = dq[db][4 * g + e] * a.scale;
-      if (d < a.D) store_vec<T, 4>(qp + d, x);
+    for (int kk = 0; kk < KK; ++kk) {
+      mfma_step<T>(lds_chunk<RB>(Qs, nb * 32 + c, 2 * kk + hf), kf[kk], s);
+      mfma_step<T>(lds_chunk<RB>(Gs, nb * 32 + c, 2 * kk + hf), vf[kk], dp);
     }
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const f32x4 st = *reinterpret_cast<const f32x4*>(St + nb * 32 + 8 * (i / 4) + 4 * hf + i % 4);   // lse, delta of two rows
+      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -st[0]));
+      s[i + 1] = __builtin_amdgcn_exp2f(fmaf(s[i + 1], c2, -st[2]));
+      dp[i] -= st[1];
+      dp[i + 1] -= st[3];
+    }
+    const int r0 = rt + nb * 32;
+    if (a.causal && group_div(r0, a.G, a.gmagic) + off < jmax) {   // (the first row of the block sees least)
+      rare_branch();
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (j > group_div(r0 + 8 * (i / 4) + 4 * hf + i % 4, a.G, a.gmagic) + off) s[i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dp[i] *= s[i];
+    accum_xt<T, D>(Gs, nb * 32, s, dv, lane);
+    accum_xt<T, D>(Qs, nb * 32, dp, dk, lane);
+  }
 }
 
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64) void packed_dkv_kernel(const PackedArgs a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D <= 64 ? 2 : 1) void packed_dkv_kernel(const PackedArgs a) {
   using F = Frag<T, D>;
-  constexpr int BM = 32 * NW, BN = 32, NT = NW * 64;   // BM keys of the workgroup, BN rows per step
-  constexpr int RB = F::RB, NC = F::NC, KK = F::KK, E = F::E;
-  __shared__ __attribute__((aligned(16))) char Qs[BN * RB];
-  __shared__ __attribute__((aligned(16))) char Gs[BN * RB];
-  __shared__ __attribute__((aligned(16))) float Ls[BN], Ds[BN];
-  __shared__ __attribute__((aligned(16))) int Lim[BN];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hf = lane >> 5, c = lane & 31;
+  constexpr int BM = 32 * NW, BN = sizeof(T) == 2 && NW > 1 ? 64 : 32, NB = BN / 32;   // BM keys, BN rows per step
+  constexpr int RB = F::RB, KK = F::KK, E = F::E, NI = BN * F::NC / (64 * NW);
+  __shared__ __attribute__((aligned(16))) char Q0[BN * RB], G0[BN * RB], Q1[BN * RB], G1[BN * RB];
+  __shared__ __attribute__((aligned(16))) float2 S0[BN], S1[BN];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5, c = lane & 31;
 
   int h, t;
   if (!head_tile(a.d, a.hkv, a.tiles, h, t)) return;
   const Seq sk = find_tile(a.cu_k, a.B, a.Mk, 1, BM, t, lane);
-  const int q0 = cu_at(a.cu_q, sk.b, a.Mq), lq = max(cu_at(a.cu_q, sk.b + 1, a.Mq) - q0, 0);
+  const int q0 = __builtin_amdgcn_readfirstlane(cu_at(a.cu_q, sk.b, a.Mq));
+  const int lq = __builtin_amdgcn_readfirstlane(max(cu_at(a.cu_q, sk.b + 1, a.Mq) - q0, 0));
   const int j0 = sk.tile * BM, off = sk.len - lq, rows = lq * a.G;
   const int store_keys = sk.b == a.B - 1 ? a.Mk - sk.start : sk.len;
   if (j0 >= store_keys) return;
-  int rbeg = 0, rend = j0 < sk.len ? rows : 0;
+  const int rend = j0 < sk.len ? rows : 0;
+  int rbeg = 0;
   if (a.causal) rbeg = (int)(min((long)rend, (long)max(0, j0 - off) * a.G) / BN) * BN;   // rows that see key j0 or later
 
-  const int j = j0 + wave * 32 + c;
+  const T* qb = (const T*)a.q + (long)q0 * a.rq + (long)h * a.G * a.hsq;
+  const T* gb = (const T*)a.dout + (long)q0 * a.rdo + (long)h * a.G * a.hsdo;
+  const float2* sb = a.rowstat + (long)q0 * a.hq + h * a.G;
+  float2 st = make_float2(0.f, 0.f);
+  // rows rt .. rt + 31 (the last one repeated) of q and dout; their statistics to registers
+  auto stage = [&](int rt, char* Qs, char* Gs) {
+    const int p0 = group_div(rt, a.G, a.gmagic);
+    const char* qt = reinterpret_cast<const char*>(qb + (long)p0 * a.rq);
+    const char* gt = reinterpret_cast<const char*>(gb + (long)p0 * a.rdo);
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      const int slot = (n * NW + wave) * 64 + lane, row = slot / F::NC, ch = (slot - row * F::NC) ^ swz<RB>(row);
+      const int rr = min(rt + row, rows - 1), pos = group_div(rr, a.G, a.gmagic);
+      const unsigned hg = (unsigned)(rr - pos * a.G), dp = (unsigned)(pos - p0), col = ch * E < a.D ? ch * 16 : 0;
+      TileCopy<T, D, BN, NW>::issue(qt + (dp * (unsigned)(a.rq * sizeof(T)) + hg * (unsigned)(a.hsq * sizeof(T)) + col), Qs + (n * NW + wave) * 1024);
+      TileCopy<T, D, BN, NW>::issue(gt + (dp * (unsigned)(a.rdo * sizeof(T)) + hg * (unsigned)(a.hsdo * sizeof(T)) + col), Gs + (n * NW + wave) * 1024);
+    }
+    if (tid < BN) {
+      const int rr = min(rt + tid, rows - 1), pos = group_div(rr, a.G, a.gmagic);
+      st = sb[(long)pos * a.hq + (rr - pos * a.G)];
+      if (rt + tid >= rows) st = make_float2(INFINITY, 0.f);   // no such row: weight 0
+    }
+  };
+  if (rbeg < rend) stage(rbeg, Q0, G0);
+
+  const int j = j0 + wave * 32 + c, jmax = j0 + wave * 32 + 31;
   const bool live = j < sk.len;
   Chunk kf[KK], vf[KK];
   {
@@ -171,83 +251,23 @@ __global__ __launch_bounds__(NW * 64) void packed_dkv_kernel(const PackedArgs a)
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) dk[db] = f32x16{}, dv[db] = f32x16{};
   const float c2 = a.scale * BLOG2E;
-  const T* qb = (const T*)a.q + (long)q0 * a.rq + (long)h * a.G * a.hsq;
-  const T* gb = (const T*)a.dout + (long)q0 * a.rdo + (long)h * a.G * a.hsdo;
 
-  for (int rt = rbeg; rt < rend; rt += BN) {
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < (BN * NC + NT - 1) / NT; ++n) {
-      const int idx = tid + n * NT;
-      if (BN * NC % NT == 0 || idx < BN * NC) {
-        const int row = idx / NC, ch = idx - row * NC, r = rt + row;
-        Chunk qc = zero_chunk(), gc = zero_chunk();
-        if (r < rows && ch * E < a.D) {
-          const int pos = group_div(r, a.G, a.gmagic), hg = r - pos * a.G;
-          qc.u = *reinterpret_cast<const uint4*>(qb + (long)pos * a.rq + (long)hg * a.hsq + ch * E);
-          gc.u = *reinterpret_cast<const uint4*>(gb + (long)pos * a.rdo + (long)hg * a.hsdo + ch * E);
-        }
-        const int at = row * RB + ((ch ^ swz<RB>(row)) << 4);
-        *reinterpret_cast<uint4*>(Qs + at) = qc.u;
-        *reinterpret_cast<uint4*>(Gs + at) = gc.u;
-      }
-    }
-    for (int i = tid; i < BN; i += NT) {
-      const int r = rt + i;
-      float lse = INFINITY, delta = 0.f;   // a row that sees nothing, or none: weights exp2(-inf) = 0
-      int lim = -1;
-      if (r < rows) {
-        const int pos = group_div(r, a.G, a.gmagic);
-        const long orow = (long)(q0 + pos) * a.hq + h * a.G + (r - pos * a.G);
-        lse = a.lse[orow] * BLOG2E;
-        if (lse == -INFINITY) lse = INFINITY;
-        delta = a.delta[orow];
-        lim = a.causal ? pos + off : sk.len;
-      }
-      Ls[i] = lse, Ds[i] = delta, Lim[i] = lim;
-    }
-    __syncthreads();
-    f32x16 s = f32x16{}, dp = f32x16{};
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      mfma_step<T>(lds_chunk<RB>(Qs, c, 2 * kk + hf), kf[kk], s);
-      mfma_step<T>(lds_chunk<RB>(Gs, c, 2 * kk + hf), vf[kk], dp);
-    }
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(Ls + 8 * g + 4 * hf);
-      const f32x4 del = *reinterpret_cast<const f32x4*>(Ds + 8 * g + 4 * hf);
-      const int4 lim = *reinterpret_cast<const int4*>(Lim + 8 * g + 4 * hf);
-      const int li[4] = {lim.x, lim.y, lim.z, lim.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = 4 * g + e;
-        float p = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -lse[e]));
-        if (j > li[e]) p = 0.f;
-        s[i] = p;
-        dp[i] = p * (dp[i] - del[e]);
-      }
-    }
-    accum_xt<T, D>(Gs, 0, s, dv, lane);
-    accum_xt<T, D>(Qs, 0, dp, dk, lane);
+  if (tid < BN) S0[tid] = st;
+  for (int rt = rbeg; rt < rend; rt += 2 * BN) {
+    tiles_ready();
+    if (rt + BN < rend) stage(rt + BN, Q1, G1);
+    dkv_tile<T, D, NB>(Q0, G0, S0, kf, vf, dk, dv, rt, off, j, jmax, a, c2, lane);
+    if (rt + BN >= rend) break;
+    if (tid < BN) S1[tid] = st;
+    tiles_ready();
+    if (rt + 2 * BN < rend) stage(rt + 2 * BN, Q0, G0);
+    dkv_tile<T, D, NB>(Q1, G1, S1, kf, vf, dk, dv, rt + BN, off, j, jmax, a, c2, lane);
+    if (tid < BN) S0[tid] = st;
   }
 
   if (j >= store_keys) return;
-  T* kp = (T*)a.dk + (long)(sk.start + j) * a.rdk + (long)h * a.hsdk;
-  T* vp = (T*)a.dv + (long)(sk.start + j) * a.rdv + (long)h * a.hsdv;
-#pragma unroll
-  for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = db * 32 + 8 * g + 4 * hf;
-      float x[4], y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = dk[db][4 * g + e] * a.scale, y[e] = dv[db][4 * g + e];
-      if (d < a.D) {
-        store_vec<T, 4>(kp + d, x);
-        store_vec<T, 4>(vp + d, y);
-      }
-    }
+  store_cols<T, D>((T*)a.dk + (long)(sk.start + j) * a.rdk + (long)h * a.hsdk, dk, a.scale, a.D, hf);
+  store_cols<T, D>((T*)a.dv + (long)(sk.start + j) * a.rdv + (long)h * a.hsdv, dv, 1.f, a.D, hf);
 }
 
 template <typename T, int D>
@@ -273,7 +293,7 @@ using namespace ogv;
 
 extern "C" size_t ogv_packed_attn_bwd_ws_bytes(const ogv_packed_desc* d, ogv_dtype dt) {
   if (packed_check("ogv_packed_attn_bwd_ws_bytes", d, dt) != OGV_OK) return 0;
-  return (size_t)d->Mq * d->heads * sizeof(float);
+  return (size_t)d->Mq * d->heads * 2 * sizeof(float);
 }
 
 extern "C" int ogv_packed_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
@@ -285,7 +305,7 @@ extern "C" int ogv_packed_attn_bwd(const void* dout, const void* q, const void* 
   OGV_REQUIRE(aligned16({dout, q, k, v, out, dq, dk, dv, ws}), "ogv_packed_attn_bwd: pointers must be 16-byte aligned");
   PackedArgs a;
   packed_args(d, a);
-  a.q = q, a.k = k, a.v = v, a.o = out, a.dout = dout, a.lse = const_cast<float*>(lse), a.delta = (float*)ws;
+  a.q = q, a.k = k, a.v = v, a.o = out, a.dout = dout, a.lse = const_cast<float*>(lse), a.rowstat = (float2*)ws;
   a.cu_q = cu_q, a.cu_k = cu_k, a.dq = dq, a.dk = dk, a.dv = dv;
   hipStream_t s = as_stream(stream);
 #define OGV_BWD(T)                                   \
