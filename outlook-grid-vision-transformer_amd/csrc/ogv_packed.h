@@ -114,6 +114,23 @@ template <int RB> __device__ __forceinline__ Chunk lds_chunk(const char* tile, i
   return c;
 }
 
+// 16 bytes a lane, from base + off (base uniform) straight to LDS: lane i's to l + 16 * i.  In assembly because the
+// compiler would make every later LDS read wait for the copy, whichever tile it writes; nothing comes back in registers,
+// and tiles_ready() below waits before anybody reads the tile.  (m0 holds the LDS address; its write needs a wait state.
+// Nothing else in these kernels uses m0.)
+__device__ __forceinline__ void copy16(const char* base, unsigned off, char* l) {
+  const unsigned at = (unsigned)(uint64_t)l;   // an LDS address is the low half of its generic one
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(off),
+               "s"(base)
+               : "memory");
+}
+
+template <typename P> __device__ __forceinline__ const char* uniform_ptr(const P* p) {
+  const uint64_t v = (uint64_t)p;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
+  return reinterpret_cast<const char*>(((uint64_t)hi << 32) | lo);
+}
+
 // Copies ROWS rows of a strided tensor into an LDS tile, straight from global memory to LDS (no registers): one
 // instruction of a wave fills 64 consecutive chunks, so the swizzle is in the addresses that the lanes read.  Rows past
 // the last one repeat it and chunks past the head repeat the first: whoever uses the tile masks their products.
@@ -133,19 +150,15 @@ template <typename T, int D, int ROWS, int NW> struct TileCopy {
   }
   // rows 0 .. ROWS - 1 behind base, of which `left` >= 1 exist
   __device__ __forceinline__ void load(const T* base, long stride, int left, char* tile, int wave, int lane, int Dlive) const {
-    const char* b = reinterpret_cast<const char*>(base);
+    const char* b = uniform_ptr(base);
     if (left >= ROWS) {
 #pragma unroll
-      for (int n = 0; n < NI; ++n) issue(b + off[n], tile + (n * NW + wave) * 1024);
+      for (int n = 0; n < NI; ++n) copy16(b, off[n], tile + (n * NW + wave) * 1024);
     } else {
 #pragma unroll
       for (int n = 0; n < NI; ++n)
-        issue(b + place((n * NW + wave) * 64 + lane, left - 1, Dlive, stride), tile + (n * NW + wave) * 1024);
+        copy16(b, place((n * NW + wave) * 64 + lane, left - 1, Dlive, stride), tile + (n * NW + wave) * 1024);
     }
-  }
-  static __device__ __forceinline__ void issue(const char* g, char* l) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
-                                     (__attribute__((address_space(3))) void*)l, 16, 0, 0);
   }
 };
 

@@ -66,8 +66,8 @@ template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dq_kernel(const PackedArgs a) {
   using F = Frag<T, D>;
   constexpr int BM = 32 * NW, BN = sizeof(T) == 2 && NW > 1 ? 64 : 32, NB = BN / 32;
-  constexpr int RB = F::RB, KK = F::KK, E = F::E;
-  __shared__ __attribute__((aligned(16))) char K0[BN * RB], V0[BN * RB], K1[BN * RB], V1[BN * RB];
+  constexpr int RB = F::RB, KK = F::KK, E = F::E, TB = BN * RB;
+  __shared__ __attribute__((aligned(16))) char tiles[4 * TB];   // K and V, two of each
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5, c = lane & 31;
 
   int h, t;
@@ -88,11 +88,11 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dq_ker
   TileCopy<T, D, BN, NW> kc, vc;
   kc.init(wave, lane, a.D, a.rk);
   vc.init(wave, lane, a.D, a.rv);
-  auto stage = [&](int kt, char* Ks, char* Vs) {
-    kc.load(kb + (long)kt * BN * a.rk, a.rk, lk - kt * BN, Ks, wave, lane, a.D);
-    vc.load(vb + (long)kt * BN * a.rv, a.rv, lk - kt * BN, Vs, wave, lane, a.D);
+  auto stage = [&](int kt, int at) {
+    kc.load(kb + (long)kt * BN * a.rk, a.rk, lk - kt * BN, tiles + at, wave, lane, a.D);
+    vc.load(vb + (long)kt * BN * a.rv, a.rv, lk - kt * BN, tiles + at + TB, wave, lane, a.D);
   };
-  if (kt1 > 0) stage(0, K0, V0);
+  if (kt1 > 0) stage(0, 0);
 
   const int r = r0 + wave * 32 + c, pos = group_div(r, a.G, a.gmagic), hg = r - pos * a.G;
   const bool live = r < rows;
@@ -134,14 +134,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dq_ker
   for (int db = 0; db < D / 32; ++db) dq[db] = f32x16{};
   const float c2 = a.scale * BLOG2E;
 
-  for (int kt = 0; kt < kt1; kt += 2) {
+  for (int kt = 0, at = 0; kt < kt1; ++kt, at ^= 2 * TB) {
     tiles_ready();
-    if (kt + 1 < kt1) stage(kt + 1, K1, V1);
-    dq_tile<T, D, NB>(K0, V0, qf, gf, dq, kt * BN, lim, c2, lse2, delta, lane);
-    if (kt + 1 >= kt1) break;
-    tiles_ready();
-    if (kt + 2 < kt1) stage(kt + 2, K0, V0);
-    dq_tile<T, D, NB>(K1, V1, qf, gf, dq, (kt + 1) * BN, lim, c2, lse2, delta, lane);
+    if (kt + 1 < kt1) stage(kt + 1, at ^ (2 * TB));
+    dq_tile<T, D, NB>(tiles + at, tiles + at + TB, qf, gf, dq, kt * BN, lim, c2, lse2, delta, lane);
   }
 
   if (r >= store_rows) return;
@@ -149,9 +145,9 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dq_ker
 }
 
 // 32 * NB rows of dk / dv: scores and dp with columns = keys, dV^T += dO^T P, dK^T += Q^T dS
-template <typename T, int D, int NB>
+template <typename T, int D, int NB, bool VL>
 __device__ __forceinline__ void dkv_tile(const char* Qs, const char* Gs, const float2* St, const Chunk (&kf)[Frag<T, D>::KK],
-                                         const Chunk (&vf)[Frag<T, D>::KK], f32x16 (&dk)[D / 32], f32x16 (&dv)[D / 32], int rt,
+                                         const Chunk (&vf)[VL ? 1 : Frag<T, D>::KK], const char* Vs, f32x16 (&dk)[D / 32], f32x16 (&dv)[D / 32], int rt,
                                          int off, int j, int jmax, const PackedArgs& a, float c2, int lane) {
   constexpr int KK = Frag<T, D>::KK, RB = Frag<T, D>::RB;
   const int hf = lane >> 5, c = lane & 31;
@@ -161,7 +157,7 @@ __device__ __forceinline__ void dkv_tile(const char* Qs, const char* Gs, const f
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       mfma_step<T>(lds_chunk<RB>(Qs, nb * 32 + c, 2 * kk + hf), kf[kk], s);
-      mfma_step<T>(lds_chunk<RB>(Gs, nb * 32 + c, 2 * kk + hf), vf[kk], dp);
+      mfma_step<T>(lds_chunk<RB>(Gs, nb * 32 + c, 2 * kk + hf), VL ? lds_chunk<RB>(Vs, c, 2 * kk + hf) : vf[VL ? 0 : kk], dp);
     }
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
@@ -185,43 +181,68 @@ __device__ __forceinline__ void dkv_tile(const char* Qs, const char* Gs, const f
   }
 }
 
+// A workgroup owns 32 * NW keys (32 per wave, K and the sums in registers) and one of a.nsplit pieces of the rows
+// that see them.  Heads of 96 and 128 keep V in LDS instead of registers: that leaves two waves to a SIMD (at one,
+// nothing covers the exponentials and the LDS reads).  One piece writes dk, dv; several write fp32 partial sums.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D <= 64 ? 2 : 1) void packed_dkv_kernel(const PackedArgs a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dkv_kernel(const PackedArgs a) {
   using F = Frag<T, D>;
-  constexpr int BM = 32 * NW, BN = sizeof(T) == 2 && NW > 1 ? 64 : 32, NB = BN / 32;   // BM keys, BN rows per step
-  constexpr int RB = F::RB, KK = F::KK, E = F::E, NI = BN * F::NC / (64 * NW);
-  __shared__ __attribute__((aligned(16))) char Q0[BN * RB], G0[BN * RB], Q1[BN * RB], G1[BN * RB];
-  __shared__ __attribute__((aligned(16))) float2 S0[BN], S1[BN];
+  constexpr bool VL = sizeof(T) == 2 && D >= 96;
+  constexpr int BM = 32 * NW, BN = sizeof(T) == 2 && NW > 1 && !VL ? 64 : 32, NB = BN / 32;   // BM keys, BN rows per step
+  constexpr int RB = F::RB, KK = F::KK, E = F::E, NT = 64 * NW, TB = BN * RB;
+  // (a step of 32 rows of a 96-wide head is one and a half instructions of four waves: the last half is left out)
+  constexpr int NI = (BN * F::NC + NT - 1) / NT;
+  __shared__ __attribute__((aligned(16))) char tiles[4 * TB];   // q and dout, two of each
+  __shared__ __attribute__((aligned(16))) char Vl[VL ? BM * RB : 16];
+  __shared__ __attribute__((aligned(16))) float2 stats[2 * BN];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5, c = lane & 31;
 
   int h, t;
-  if (!head_tile(a.d, a.hkv, a.tiles, h, t)) return;
-  const Seq sk = find_tile(a.cu_k, a.B, a.Mk, 1, BM, t, lane);
+  if (!head_tile(a.d, a.hkv, a.tiles * a.nsplit, h, t)) return;
+  const int split = t % a.nsplit;
+  const Seq sk = find_tile(a.cu_k, a.B, a.Mk, 1, BM, t / a.nsplit, lane);
   const int q0 = __builtin_amdgcn_readfirstlane(cu_at(a.cu_q, sk.b, a.Mq));
   const int lq = __builtin_amdgcn_readfirstlane(max(cu_at(a.cu_q, sk.b + 1, a.Mq) - q0, 0));
   const int j0 = sk.tile * BM, off = sk.len - lq, rows = lq * a.G;
   const int store_keys = sk.b == a.B - 1 ? a.Mk - sk.start : sk.len;
   if (j0 >= store_keys) return;
-  const int rend = j0 < sk.len ? rows : 0;
-  int rbeg = 0;
+  int rend = j0 < sk.len ? rows : 0, rbeg = 0;
   if (a.causal) rbeg = (int)(min((long)rend, (long)max(0, j0 - off) * a.G) / BN) * BN;   // rows that see key j0 or later
+  if (a.nsplit > 1) {
+    const int per = ((rend - rbeg + a.nsplit - 1) / a.nsplit + BN - 1) / BN * BN;
+    rbeg = min(rbeg + split * per, rend);
+    rend = min(rbeg + per, rend);
+  }
 
   const T* qb = (const T*)a.q + (long)q0 * a.rq + (long)h * a.G * a.hsq;
   const T* gb = (const T*)a.dout + (long)q0 * a.rdo + (long)h * a.G * a.hsdo;
   const float2* sb = a.rowstat + (long)q0 * a.hq + h * a.G;
   float2 st = make_float2(0.f, 0.f);
-  // rows rt .. rt + 31 (the last one repeated) of q and dout; their statistics to registers
-  auto stage = [&](int rt, char* Qs, char* Gs) {
+  // byte offsets of a lane's chunks from row rt's query, for rr = rt + row clamped by the caller
+  auto place = [&](int n, int rt, int p0, int last, unsigned& oq, unsigned& og) {
+    const int slot = (n * NW + wave) * 64 + lane, row = slot / F::NC, ch = (slot - row * F::NC) ^ swz<RB>(row);
+    const int rr = min(rt + row, last), pos = group_div(rr, a.G, a.gmagic);
+    const unsigned hg = (unsigned)(rr - pos * a.G), dp = (unsigned)(pos - p0), col = ch * E < a.D ? ch * 16 : 0;
+    oq = dp * (unsigned)(a.rq * sizeof(T)) + hg * (unsigned)(a.hsq * sizeof(T)) + col;
+    og = dp * (unsigned)(a.rdo * sizeof(T)) + hg * (unsigned)(a.hsdo * sizeof(T)) + col;
+  };
+  unsigned oq[NI], og[NI];   // of a whole step whose first row is its query's first head (always, where G divides BN)
+#pragma unroll
+  for (int n = 0; n < NI; ++n) place(n, 0, 0, BN, oq[n], og[n]);
+  const bool even = BN % a.G == 0;
+  // rows rt .. rt + BN - 1 (the last one repeated) of q and dout to LDS; their statistics to registers
+  auto stage = [&](int rt, int at) {
     const int p0 = group_div(rt, a.G, a.gmagic);
-    const char* qt = reinterpret_cast<const char*>(qb + (long)p0 * a.rq);
-    const char* gt = reinterpret_cast<const char*>(gb + (long)p0 * a.rdo);
+    const char* qt = uniform_ptr(qb + (long)p0 * a.rq);
+    const char* gt = uniform_ptr(gb + (long)p0 * a.rdo);
+    const bool whole = even && rt + BN <= rows;
 #pragma unroll
     for (int n = 0; n < NI; ++n) {
-      const int slot = (n * NW + wave) * 64 + lane, row = slot / F::NC, ch = (slot - row * F::NC) ^ swz<RB>(row);
-      const int rr = min(rt + row, rows - 1), pos = group_div(rr, a.G, a.gmagic);
-      const unsigned hg = (unsigned)(rr - pos * a.G), dp = (unsigned)(pos - p0), col = ch * E < a.D ? ch * 16 : 0;
-      TileCopy<T, D, BN, NW>::issue(qt + (dp * (unsigned)(a.rq * sizeof(T)) + hg * (unsigned)(a.hsq * sizeof(T)) + col), Qs + (n * NW + wave) * 1024);
-      TileCopy<T, D, BN, NW>::issue(gt + (dp * (unsigned)(a.rdo * sizeof(T)) + hg * (unsigned)(a.hsdo * sizeof(T)) + col), Gs + (n * NW + wave) * 1024);
+      if (BN * F::NC % NT != 0 && (n * NW + wave) * 64 >= BN * F::NC) break;   // (uniform in a wave)
+      unsigned x = oq[n], y = og[n];
+      if (!whole) place(n, rt, p0, rows - 1, x, y);
+      copy16(qt, x, tiles + at + (n * NW + wave) * 1024);
+      copy16(gt, y, tiles + at + TB + (n * NW + wave) * 1024);
     }
     if (tid < BN) {
       const int rr = min(rt + tid, rows - 1), pos = group_div(rr, a.G, a.gmagic);
@@ -229,21 +250,33 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D <= 64 ? 2 : 1) void pa
       if (rt + tid >= rows) st = make_float2(INFINITY, 0.f);   // no such row: weight 0
     }
   };
-  if (rbeg < rend) stage(rbeg, Q0, G0);
-
   const int j = j0 + wave * 32 + c, jmax = j0 + wave * 32 + 31;
   const bool live = j < sk.len;
-  Chunk kf[KK], vf[KK];
-  {
-    const T* kp = (const T*)a.k + (long)(sk.start + (live ? j : 0)) * a.rk + (long)h * a.hsk;
-    const T* vp = (const T*)a.v + (long)(sk.start + (live ? j : 0)) * a.rv + (long)h * a.hsv;
+  Chunk kf[KK], vf[VL ? 1 : KK];
+  if (rbeg < rend) {
+    stage(rbeg, 0);
+    if constexpr (VL) {
+      TileCopy<T, D, BM, NW> vc;
+      vc.init(wave, lane, a.D, a.rv);
+      vc.load((const T*)a.v + (long)(sk.start + j0) * a.rv + (long)h * a.hsv, a.rv, sk.len - j0, Vl, wave, lane, a.D);
+      if (a.D < D) {   // dout's chunks past the head are not zero, so these have to be
+        tiles_ready();
+        for (int i = tid; i < BM * F::NC; i += NT) {
+          const int row = i / F::NC, ch = i - row * F::NC;
+          if (ch * E >= a.D) *reinterpret_cast<uint4*>(Vl + row * RB + ((ch ^ swz<RB>(row)) << 4)) = make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+    const T* kp = (const T*)a.k + (long)(sk.start + (live ? j : j0)) * a.rk + (long)h * a.hsk;
+    const T* vp = (const T*)a.v + (long)(sk.start + (live ? j : j0)) * a.rv + (long)h * a.hsv;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       const int d = (2 * kk + hf) * E;
-      kf[kk] = vf[kk] = zero_chunk();
-      if (live && d < a.D) {
-        kf[kk].u = *reinterpret_cast<const uint4*>(kp + d);
-        vf[kk].u = *reinterpret_cast<const uint4*>(vp + d);
+      kf[kk] = zero_chunk();
+      if (d < a.D) kf[kk].u = *reinterpret_cast<const uint4*>(kp + d);
+      if constexpr (!VL) {
+        vf[kk] = zero_chunk();
+        if (d < a.D) vf[kk].u = *reinterpret_cast<const uint4*>(vp + d);
       }
     }
   }
@@ -251,40 +284,85 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D <= 64 ? 2 : 1) void pa
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) dk[db] = f32x16{}, dv[db] = f32x16{};
   const float c2 = a.scale * BLOG2E;
+  const char* Vw = Vl + (VL ? wave * 32 * RB : 0);
 
-  if (tid < BN) S0[tid] = st;
-  for (int rt = rbeg; rt < rend; rt += 2 * BN) {
+  for (int rt = rbeg, at = 0; rt < rend; rt += BN, at ^= 2 * TB) {
+    float2* S = stats + (at ? BN : 0);
+    if (tid < BN) S[tid] = st;
     tiles_ready();
-    if (rt + BN < rend) stage(rt + BN, Q1, G1);
-    dkv_tile<T, D, NB>(Q0, G0, S0, kf, vf, dk, dv, rt, off, j, jmax, a, c2, lane);
-    if (rt + BN >= rend) break;
-    if (tid < BN) S1[tid] = st;
-    tiles_ready();
-    if (rt + 2 * BN < rend) stage(rt + 2 * BN, Q0, G0);
-    dkv_tile<T, D, NB>(Q1, G1, S1, kf, vf, dk, dv, rt + BN, off, j, jmax, a, c2, lane);
-    if (tid < BN) S0[tid] = st;
+    if (rt + BN < rend) stage(rt + BN, at ^ (2 * TB));
+    dkv_tile<T, D, NB, VL>(tiles + at, tiles + at + TB, S, kf, vf, Vw, dk, dv, rt, off, j, jmax, a, c2, lane);
   }
 
   if (j >= store_keys) return;
+  if (!live) {   // keys behind the last sequence
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) dk[db] = f32x16{}, dv[db] = f32x16{};
+  }
+  if (a.nsplit > 1) {
+    const long n = (long)a.Mk * a.hkv, row = (long)(sk.start + j) * a.hkv + h;
+    store_cols<float, D>(a.part_o + ((2L * split) * n + row) * a.D, dk, 1.f, a.D, hf);
+    store_cols<float, D>(a.part_o + ((2L * split + 1) * n + row) * a.D, dv, 1.f, a.D, hf);
+    return;
+  }
   store_cols<T, D>((T*)a.dk + (long)(sk.start + j) * a.rdk + (long)h * a.hsdk, dk, a.scale, a.D, hf);
   store_cols<T, D>((T*)a.dv + (long)(sk.start + j) * a.rdv + (long)h * a.hsdv, dv, 1.f, a.D, hf);
 }
 
+// dk, dv = sums of the row pieces, in order
+template <typename T>
+__global__ __launch_bounds__(256) void packed_sum_kernel(const PackedArgs a) {
+  const int per = a.D / 4;
+  const long n = (long)a.Mk * a.hkv, idx = (long)blockIdx.x * 256 + threadIdx.x;
+  if (idx >= 2 * n * per) return;
+  const long row2 = idx / per, row = row2 >> 1, key = row / a.hkv;   // dk and dv of a row next to each other
+  const int d = (int)(idx - row2 * per) * 4, which = (int)(row2 & 1), h = (int)(row - key * a.hkv);
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float4 p = *reinterpret_cast<const float4*>(a.part_o + ((2L * s + which) * n + row) * a.D + d);
+    x[0] += p.x, x[1] += p.y, x[2] += p.z, x[3] += p.w;
+  }
+  const float mul = which ? 1.f : a.scale;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] *= mul;
+  T* out = which ? (T*)a.dv + key * a.rdv + h * a.hsdv : (T*)a.dk + key * a.rdk + h * a.hsdk;
+  store_vec<T, 4>(out + d, x);
+}
+
+struct BwdPlan {
+  int nwq, nwk, tiles_q, tiles_k, nsplit;
+};
+
+// Waves per workgroup as in the forward.  The rows of dk / dv are split while the key tiles would not fill the 256 CUs
+// three times (under the causal mask the first tile has twice the average work), at least 512 rows to a piece: a piece
+// costs 16 bytes of partial sums per key, head and dim.
+static BwdPlan bwd_plan(const ogv_packed_desc* d) {
+  BwdPlan p;
+  const long rows = (long)d->Mq * (d->heads / d->kv_heads);
+  p.nwq = rows >= 96L * d->B ? 4 : 1, p.nwk = d->Mk >= 96L * d->B ? 4 : 1;
+  p.tiles_q = (int)(rows / (32 * p.nwq)) + d->B;
+  p.tiles_k = d->Mk / (32 * p.nwk) + d->B;
+  const long blocks = (long)p.tiles_k * d->kv_heads;
+  long n = blocks < 512 ? (768 + blocks - 1) / blocks : 1;
+  const long most = rows / d->B / 512;
+  if (n > most) n = most;
+  p.nsplit = (int)(n < 1 ? 1 : n > 16 ? 16 : n);
+  return p;
+}
+
 template <typename T, int D>
-static void bwd_launch(PackedArgs a, hipStream_t s) {
-  const long rows = (long)a.Mq * a.G;
-  const int nwq = rows >= 96L * a.B ? 4 : 1, nwk = a.Mk >= 96L * a.B ? 4 : 1;
-  a.tiles = (int)(rows / (32 * nwq)) + a.B;
-  a.d = deal(a.hkv, a.tiles);
+static void bwd_launch(const BwdPlan& p, PackedArgs a, hipStream_t s) {
+  a.tiles = p.tiles_q, a.d = deal(a.hkv, a.tiles);
   const unsigned nq = deal_grid(a.hkv, a.tiles);
-  if (nwq == 4) packed_dq_kernel<T, D, 4><<<nq, 256, 0, s>>>(a);
+  if (p.nwq == 4) packed_dq_kernel<T, D, 4><<<nq, 256, 0, s>>>(a);
   else packed_dq_kernel<T, D, 1><<<nq, 64, 0, s>>>(a);
   if (a.Mk == 0) return;
-  a.tiles = a.Mk / (32 * nwk) + a.B;
-  a.d = deal(a.hkv, a.tiles);
-  const unsigned nk = deal_grid(a.hkv, a.tiles);
-  if (nwk == 4) packed_dkv_kernel<T, D, 4><<<nk, 256, 0, s>>>(a);
+  a.tiles = p.tiles_k, a.nsplit = p.nsplit, a.d = deal(a.hkv, a.tiles * a.nsplit);
+  const unsigned nk = deal_grid(a.hkv, a.tiles * a.nsplit);
+  if (p.nwk == 4) packed_dkv_kernel<T, D, 4><<<nk, 256, 0, s>>>(a);
   else packed_dkv_kernel<T, D, 1><<<nk, 64, 0, s>>>(a);
+  if (a.nsplit > 1) packed_sum_kernel<T><<<cdiv((long)a.Mk * a.hkv * (a.D / 2), 256), 256, 0, s>>>(a);
 }
 
 }  // namespace ogv
@@ -293,7 +371,9 @@ using namespace ogv;
 
 extern "C" size_t ogv_packed_attn_bwd_ws_bytes(const ogv_packed_desc* d, ogv_dtype dt) {
   if (packed_check("ogv_packed_attn_bwd_ws_bytes", d, dt) != OGV_OK) return 0;
-  return (size_t)d->Mq * d->heads * 2 * sizeof(float);
+  const BwdPlan p = bwd_plan(d);
+  const size_t stat = ((size_t)d->Mq * d->heads * 2 + 3) & ~(size_t)3;
+  return (stat + (p.nsplit > 1 ? (size_t)p.nsplit * 2 * d->Mk * d->kv_heads * d->D : 0)) * sizeof(float);
 }
 
 extern "C" int ogv_packed_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
@@ -307,12 +387,14 @@ extern "C" int ogv_packed_attn_bwd(const void* dout, const void* q, const void* 
   packed_args(d, a);
   a.q = q, a.k = k, a.v = v, a.o = out, a.dout = dout, a.lse = const_cast<float*>(lse), a.rowstat = (float2*)ws;
   a.cu_q = cu_q, a.cu_k = cu_k, a.dq = dq, a.dk = dk, a.dv = dv;
+  a.part_o = (float*)ws + (((size_t)d->Mq * d->heads * 2 + 3) & ~(size_t)3);
+  const BwdPlan p = bwd_plan(d);
   hipStream_t s = as_stream(stream);
-#define OGV_BWD(T)                                   \
-  if (d->D <= 32) bwd_launch<T, 32>(a, s);           \
-  else if (d->D <= 64) bwd_launch<T, 64>(a, s);      \
-  else if (d->D <= 96) bwd_launch<T, 96>(a, s);      \
-  else bwd_launch<T, 128>(a, s);
+#define OGV_BWD(T)                                      \
+  if (d->D <= 32) bwd_launch<T, 32>(p, a, s);           \
+  else if (d->D <= 64) bwd_launch<T, 64>(p, a, s);      \
+  else if (d->D <= 96) bwd_launch<T, 96>(p, a, s);      \
+  else bwd_launch<T, 128>(p, a, s);
   if (dt == OGV_BF16) { OGV_BWD(bf16) } else { OGV_BWD(float) }
 #undef OGV_BWD
   return check_launch("ogv_packed_attn_bwd");

@@ -84,10 +84,10 @@ __device__ __forceinline__ void fwd_tile(const char* Ks, const char* Vs, const C
 
 // One row tile over keys kt0 * BN .. of its sequence.
 template <typename T, int D, int NW, bool SPLIT>
-__device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* K0, char* V0, char* K1, char* V1, int h, int b, int tile, int piece) {
+__device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* tiles, int h, int b, int tile, int piece) {
   using F = Frag<T, D>;
   constexpr int BM = 32 * NW, BN = sizeof(T) == 2 && NW > 1 ? 64 : 32, NB = BN / 32;
-  constexpr int KK = F::KK, E = F::E;
+  constexpr int KK = F::KK, E = F::E, TB = BN * F::RB;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5, c = lane & 31;
   const int start = __builtin_amdgcn_readfirstlane(cu_at(a.cu_q, b, a.Mq));
   const int len = __builtin_amdgcn_readfirstlane(max(cu_at(a.cu_q, b + 1, a.Mq) - start, 0));
@@ -113,11 +113,12 @@ __device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* K0, char* V0
   TileCopy<T, D, BN, NW> kc, vc;
   kc.init(wave, lane, a.D, a.rk);
   vc.init(wave, lane, a.D, a.rv);
-  auto stage = [&](int kt, char* Ks, char* Vs) {
-    kc.load(kb + (long)kt * BN * a.rk, a.rk, lk - kt * BN, Ks, wave, lane, a.D);
-    vc.load(vb + (long)kt * BN * a.rv, a.rv, lk - kt * BN, Vs, wave, lane, a.D);
+  // K and V tiles, two of each: the next is under way while one is used
+  auto stage = [&](int kt, int at) {
+    kc.load(kb + (long)kt * BN * a.rk, a.rk, lk - kt * BN, tiles + at, wave, lane, a.D);
+    vc.load(vb + (long)kt * BN * a.rv, a.rv, lk - kt * BN, tiles + at + TB, wave, lane, a.D);
   };
-  if (kt0 < kt1) stage(kt0, K0, V0);
+  if (kt0 < kt1) stage(kt0, 0);
 
   const int r = r0 + wave * 32 + c, pos = group_div(r, a.G, a.gmagic), hg = r - pos * a.G;
   const bool live = r < rows;
@@ -138,15 +139,10 @@ __device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* K0, char* V0
   float m = -INFINITY, l = 0.f;   // m: of q . k, before the scale; l: this lane's half of the row
   const float c2 = a.scale * LOG2E, grow = 8.f / c2;
 
-  // two tiles of LDS: the next tile is under way while this one is used
-  for (int kt = kt0; kt < kt1; kt += 2) {
+  for (int kt = kt0, at = 0; kt < kt1; ++kt, at ^= 2 * TB) {
     tiles_ready();
-    if (kt + 1 < kt1) stage(kt + 1, K1, V1);
-    fwd_tile<T, D, NB>(K0, V0, qf, o, m, l, kt * BN, lim, c2, grow, lane);
-    if (kt + 1 >= kt1) break;
-    tiles_ready();
-    if (kt + 2 < kt1) stage(kt + 2, K0, V0);
-    fwd_tile<T, D, NB>(K1, V1, qf, o, m, l, (kt + 1) * BN, lim, c2, grow, lane);
+    if (kt + 1 < kt1) stage(kt + 1, at ^ (2 * TB));
+    fwd_tile<T, D, NB>(tiles + at, tiles + at + TB, qf, o, m, l, kt * BN, lim, c2, grow, lane);
   }
 
   l += __shfl_xor(l, 32, 64);
@@ -186,20 +182,20 @@ __device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* K0, char* V0
 template <typename T, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_fwd_kernel(const PackedArgs a) {
   constexpr int TB = (sizeof(T) == 2 && NW > 1 ? 64 : 32) * Frag<T, D>::RB;
-  __shared__ __attribute__((aligned(16))) char K0[TB], V0[TB], K1[TB], V1[TB];
+  __shared__ __attribute__((aligned(16))) char tiles[4 * TB];
   const int lane = threadIdx.x & 63;
   if (SPLIT) {   // every piece of work, head by head
     for (int n = blockIdx.x;; n += gridDim.x) {
       Piece p;
       if (!find_piece(a, 32 * NW, n / a.hkv, lane, p)) return;
-      fwd_rows<T, D, NW, true>(a, K0, V0, K1, V1, n % a.hkv, p.b, p.tile, p.piece);
+      fwd_rows<T, D, NW, true>(a, tiles, n % a.hkv, p.b, p.tile, p.piece);
       __syncthreads();   // the tiles are free again
     }
   } else {
     int h, t;
     if (!head_tile(a.d, a.hkv, a.tiles, h, t)) return;
     const Seq sq = find_tile(a.cu_q, a.B, a.Mq, a.G, 32 * NW, a.tiles - 1 - t, lane);
-    fwd_rows<T, D, NW, false>(a, K0, V0, K1, V1, h, sq.b, sq.tile, 0);
+    fwd_rows<T, D, NW, false>(a, tiles, h, sq.b, sq.tile, 0);
   }
 }
 

@@ -101,6 +101,22 @@ def test_attention_few_rows_many_keys(dtype, lq, lk, h, hkv):
         _check(q, k, v, lq, lk, causal, dout=do)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=str)
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("h,hkv,lengths", [(3, 1, (900, 700)), (4, 1, (1100,)), (2, 2, (1400, 1700))], ids=str)
+def test_attention_rows_split_for_keys(dtype, D, h, hkv, lengths):
+    """Few key tiles and many rows: the rows of dk and dv are split between workgroups and their sums joined."""
+    import ctypes
+
+    import ogv._lib as L
+    m = sum(lengths)
+    d = L.PackedDesc(B=len(lengths), Mq=m, Mk=m, heads=h, kv_heads=hkv, D=D, scale=1.0)
+    assert L.load().ogv_packed_attn_bwd_ws_bytes(ctypes.byref(d), 1 if dtype == BF else 0) > 8 * m * h + 16
+    q, k, v, do = _qkv(m, m, h, hkv, D, dtype, D + h)
+    for causal in (False, True):
+        _check(q, k, v, lengths, lengths, causal, dout=do)
+
+
 def test_attention_layouts():
     """Slices of one projection, head-major tensors, unaligned ones, broadcast heads: the same bits as contiguous ones."""
     from ogv.packed import packed_attention
@@ -136,8 +152,9 @@ def test_attention_layouts():
         assert (x.float() - y.float()).abs().max() <= 8 * 2.0**-8 * y.float().abs().max()
 
 
+@pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("dtype", [BF, F32], ids=str)
-def test_attention_rows_behind_the_last_sequence(dtype):
+def test_attention_rows_behind_the_last_sequence(dtype, causal):
     """Rows that belong to no sequence hold NaN: they give zeros and reach nothing; so does another sequence's NaN."""
     lengths, pad = (33, 70), 150
     q, k, v, do = _qkv(103, 103, 4, 2, 40, dtype, 9)
@@ -148,9 +165,9 @@ def test_attention_rows_behind_the_last_sequence(dtype):
         return torch.cat([t, torch.full((pad, *t.shape[1:]), math.nan, dtype=dtype)]).to(DEV).requires_grad_()
 
     qd, kd, vd = tail(q), tail(k), tail(v)
-    out, lse = packed_attention(qd, kd, vd, cu, causal=True, return_lse=True)
+    out, lse = packed_attention(qd, kd, vd, cu, causal=causal, return_lse=True)
     got = torch.autograd.grad(out, (qd, kd, vd), tail(do).detach())
-    want = _check(q, k, v, lengths, lengths, True, dout=do)
+    want = _check(q, k, v, lengths, lengths, causal, dout=do)
     for a, b in zip((out, *got), want):
         assert torch.equal(a[:103], b) and (a[103:] == 0).all()
     assert (lse[103:] == -math.inf).all()
@@ -159,7 +176,7 @@ def test_attention_rows_behind_the_last_sequence(dtype):
         t[5] = math.nan
         t[7] = math.inf
     qd, kd, vd = (t.to(DEV).requires_grad_() for t in (q, k, v))
-    out = packed_attention(qd, kd, vd, cu, causal=True)
+    out = packed_attention(qd, kd, vd, cu, causal=causal)
     got = torch.autograd.grad(out, (qd, kd, vd), do.to(DEV))
     for a, b in zip((out, *got), want):
         assert torch.equal(a[33:], b[33:])
