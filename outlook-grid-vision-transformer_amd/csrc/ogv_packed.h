@@ -221,26 +221,39 @@ __device__ __forceinline__ void accum_xt(const char* tile, int row0, const f32x1
 // M * G / BM + B.  A whole wave searches (64 probes a round).  Offsets are clamped to [0, M], the first one
 // to 0, so a bad offset array cannot lead outside the tensors.
 struct Seq {
-  int b, tile, start, len;
+  int b, tile, start, len, start2, len2;   // rows of the tiled side, rows of the other side
 };
 __device__ __forceinline__ int cu_at(const int* __restrict__ cu, int b, int M) {
   return b <= 0 ? 0 : min(max(cu[b], 0), M);
 }
-__device__ __forceinline__ Seq find_tile(const int* __restrict__ cu, int B, int M, int G, int BM, int t, int lane) {
-  int lo = 0, n = B;   // the answer is in [lo, lo + n)
-  while (n > 1) {
-    const int step = (n + 63) >> 6, idx = lo + lane * step;
-    const bool ok = lane * step < n && (int)(((long)cu_at(cu, idx, M) * G) / BM) + idx <= t;
-    const int hits = __popcll(__ballot(ok));
-    const int j = hits > 0 ? hits - 1 : 0;
-    n = min(step, n - j * step);
-    lo += j * step;
-  }
+// cu / M: the side that is tiled, G * its rows in tiles of BM; cu2 / M2: the other side
+__device__ __forceinline__ Seq find_tile(const int* __restrict__ cu, const int* __restrict__ cu2, int B, int M, int M2, int G, int BM,
+                                         int t, int lane) {
   Seq s;
-  s.b = __builtin_amdgcn_readfirstlane(lo);
-  s.start = __builtin_amdgcn_readfirstlane(cu_at(cu, s.b, M));
-  s.len = __builtin_amdgcn_readfirstlane(max(cu_at(cu, s.b + 1, M) - s.start, 0));
-  s.tile = t - ((int)(((long)s.start * G) / BM) + s.b);
+  int at, end, at2, end2;
+  if (B < 64) {   // the offsets fit a wave: one load each, everything else from registers
+    const int x = cu_at(cu, min(lane, B), M), y = cu_at(cu2, min(lane, B), M2);
+    const bool ok = lane < B && (int)(((long)x * G) / BM) + lane <= t;
+    const int hits = __popcll(__ballot(ok));
+    s.b = __builtin_amdgcn_readfirstlane(hits > 0 ? hits - 1 : 0);
+    at = __builtin_amdgcn_readlane(x, s.b), end = __builtin_amdgcn_readlane(x, s.b + 1);
+    at2 = __builtin_amdgcn_readlane(y, s.b), end2 = __builtin_amdgcn_readlane(y, s.b + 1);
+  } else {
+    int lo = 0, n = B;   // the answer is in [lo, lo + n)
+    while (n > 1) {
+      const int step = (n + 63) >> 6, idx = lo + lane * step;
+      const bool ok = lane * step < n && (int)(((long)cu_at(cu, idx, M) * G) / BM) + idx <= t;
+      const int hits = __popcll(__ballot(ok));
+      const int j = hits > 0 ? hits - 1 : 0;
+      n = min(step, n - j * step);
+      lo += j * step;
+    }
+    s.b = __builtin_amdgcn_readfirstlane(lo);
+    at = __builtin_amdgcn_readfirstlane(cu_at(cu, s.b, M)), end = __builtin_amdgcn_readfirstlane(cu_at(cu, s.b + 1, M));
+    at2 = __builtin_amdgcn_readfirstlane(cu_at(cu2, s.b, M2)), end2 = __builtin_amdgcn_readfirstlane(cu_at(cu2, s.b + 1, M2));
+  }
+  s.start = at, s.len = max(end - at, 0), s.start2 = at2, s.len2 = max(end2 - at2, 0);
+  s.tile = t - ((int)(((long)at * G) / BM) + s.b);
   return s;
 }
 
@@ -252,17 +265,19 @@ __device__ __forceinline__ int piece_keys(int lk, int chunk, int most) {
 // Work item t of the split forward = (sequence, row tile, key piece), sequences in order, a sequence's pieces of
 // one row tile next to each other.  Returns false past the last item.  The whole wave searches, 64 sequences at a time.
 struct Piece {
-  int b, tile, piece;
+  Seq s;
+  int piece;
 };
 __device__ __forceinline__ bool find_piece(const PackedArgs& a, int BM, int t, int lane, Piece& p) {
   int base = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
-    int n = 0, pieces = 1;
+    int n = 0, pieces = 1, q0 = 0, k0 = 0, len = 0, lk = 0;
     if (b < a.B) {
-      const int q0 = cu_at(a.cu_q, b, a.Mq), k0 = cu_at(a.cu_k, b, a.Mk);
-      const int lq = max((b == a.B - 1 ? a.Mq : cu_at(a.cu_q, b + 1, a.Mq)) - q0, 0);   // the last one's rows and those behind
-      const int lk = max(cu_at(a.cu_k, b + 1, a.Mk) - k0, 0);
+      q0 = cu_at(a.cu_q, b, a.Mq), k0 = cu_at(a.cu_k, b, a.Mk);
+      len = max(cu_at(a.cu_q, b + 1, a.Mq) - q0, 0);
+      lk = max(cu_at(a.cu_k, b + 1, a.Mk) - k0, 0);
+      const int lq = b == a.B - 1 ? a.Mq - q0 : len;   // the last one's rows and those behind
       const int keys = piece_keys(lk, a.chunk, a.nsplit);
       pieces = max(1, (lk + keys - 1) / keys);
       n = (int)(((long)lq * a.G + BM - 1) / BM) * pieces;
@@ -277,8 +292,10 @@ __device__ __forceinline__ bool find_piece(const PackedArgs& a, int BM, int t, i
     if (over) {
       const int w = __builtin_ctzll(over);
       const int item = t - (base + __shfl(sum - n, w, 64)), pw = __shfl(pieces, w, 64);
-      p.b = __builtin_amdgcn_readfirstlane(b0 + w);
-      p.tile = __builtin_amdgcn_readfirstlane(item / pw);
+      p.s.b = __builtin_amdgcn_readfirstlane(b0 + w);
+      p.s.tile = __builtin_amdgcn_readfirstlane(item / pw);
+      p.s.start = __builtin_amdgcn_readlane(q0, w), p.s.len = __builtin_amdgcn_readlane(len, w);
+      p.s.start2 = __builtin_amdgcn_readlane(k0, w), p.s.len2 = __builtin_amdgcn_readlane(lk, w);
       p.piece = __builtin_amdgcn_readfirstlane(item % pw);
       return true;
     }

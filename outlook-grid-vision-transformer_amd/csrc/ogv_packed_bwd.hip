@@ -72,9 +72,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dq_ker
 
   int h, t;
   if (!head_tile(a.d, a.hkv, a.tiles, h, t)) return;
-  const Seq sq = find_tile(a.cu_q, a.B, a.Mq, a.G, BM, a.tiles - 1 - t, lane);
-  const int k0 = __builtin_amdgcn_readfirstlane(cu_at(a.cu_k, sq.b, a.Mk));
-  const int lk = __builtin_amdgcn_readfirstlane(max(cu_at(a.cu_k, sq.b + 1, a.Mk) - k0, 0));
+  const Seq sq = find_tile(a.cu_q, a.cu_k, a.B, a.Mq, a.Mk, a.G, BM, a.tiles - 1 - t, lane);
+  const int k0 = sq.start2, lk = sq.len2;
   const int rows = sq.len * a.G, r0 = sq.tile * BM;
   const int store_rows = sq.b == a.B - 1 ? (a.Mq - sq.start) * a.G : rows;
   if (r0 >= store_rows) return;
@@ -200,9 +199,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dkv_ke
   int h, t;
   if (!head_tile(a.d, a.hkv, a.tiles * a.nsplit, h, t)) return;
   const int split = t % a.nsplit;
-  const Seq sk = find_tile(a.cu_k, a.B, a.Mk, 1, BM, t / a.nsplit, lane);
-  const int q0 = __builtin_amdgcn_readfirstlane(cu_at(a.cu_q, sk.b, a.Mq));
-  const int lq = __builtin_amdgcn_readfirstlane(max(cu_at(a.cu_q, sk.b + 1, a.Mq) - q0, 0));
+  const Seq sk = find_tile(a.cu_k, a.cu_q, a.B, a.Mk, a.Mq, 1, BM, t / a.nsplit, lane);
+  const int q0 = sk.start2, lq = sk.len2;
   const int j0 = sk.tile * BM, off = sk.len - lq, rows = lq * a.G;
   const int store_keys = sk.b == a.B - 1 ? a.Mk - sk.start : sk.len;
   if (j0 >= store_keys) return;

@@ -84,16 +84,13 @@ __device__ __forceinline__ void fwd_tile(const char* Ks, const char* Vs, const C
 
 // One row tile over keys kt0 * BN .. of its sequence.
 template <typename T, int D, int NW, bool SPLIT>
-__device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* tiles, int h, int b, int tile, int piece) {
+__device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* tiles, int h, const Seq& sq, int piece) {
   using F = Frag<T, D>;
   constexpr int BM = 32 * NW, BN = sizeof(T) == 2 && NW > 1 ? 64 : 32, NB = BN / 32;
   constexpr int KK = F::KK, E = F::E, TB = BN * F::RB;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5, c = lane & 31;
-  const int start = __builtin_amdgcn_readfirstlane(cu_at(a.cu_q, b, a.Mq));
-  const int len = __builtin_amdgcn_readfirstlane(max(cu_at(a.cu_q, b + 1, a.Mq) - start, 0));
-  const int k0 = __builtin_amdgcn_readfirstlane(cu_at(a.cu_k, b, a.Mk));
-  const int lk = __builtin_amdgcn_readfirstlane(max(cu_at(a.cu_k, b + 1, a.Mk) - k0, 0));
-  const int rows = len * a.G, r0 = tile * BM;
+  const int b = sq.b, start = sq.start, len = sq.len, k0 = sq.start2, lk = sq.len2;
+  const int rows = len * a.G, r0 = sq.tile * BM;
   // rows behind the last sequence belong to nothing: zeros
   const int store_rows = b == a.B - 1 ? (a.Mq - start) * a.G : rows;
   if (r0 >= store_rows) return;
@@ -188,14 +185,14 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_fwd_ke
     for (int n = blockIdx.x;; n += gridDim.x) {
       Piece p;
       if (!find_piece(a, 32 * NW, n / a.hkv, lane, p)) return;
-      fwd_rows<T, D, NW, true>(a, tiles, n % a.hkv, p.b, p.tile, p.piece);
+      fwd_rows<T, D, NW, true>(a, tiles, n % a.hkv, p.s, p.piece);
       __syncthreads();   // the tiles are free again
     }
   } else {
     int h, t;
     if (!head_tile(a.d, a.hkv, a.tiles, h, t)) return;
-    const Seq sq = find_tile(a.cu_q, a.B, a.Mq, a.G, 32 * NW, a.tiles - 1 - t, lane);
-    fwd_rows<T, D, NW, false>(a, tiles, h, sq.b, sq.tile, 0);
+    const Seq sq = find_tile(a.cu_q, a.cu_k, a.B, a.Mq, a.Mk, a.G, 32 * NW, a.tiles - 1 - t, lane);
+    fwd_rows<T, D, NW, false>(a, tiles, h, sq, 0);
   }
 }
 
