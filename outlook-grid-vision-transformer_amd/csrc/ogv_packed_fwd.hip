@@ -15,21 +15,29 @@
 
 namespace ogv {
 
+#ifndef OGV_INTERLEAVE
+#define OGV_INTERLEAVE
+#endif
 constexpr float LOG2E = 1.4426950408889634f;
 
-// One tile of keys: scores, running maximum and sum, O += P V.
+// S^T = K Q^T of one key tile.
 template <typename T, int D, int NB>
-__device__ __forceinline__ void fwd_tile(const char* Ks, const char* Vs, const Chunk (&qf)[Frag<T, D>::KK], f32x16 (&o)[D / 32],
-                                         float& m, float& l, int key0, int lim, float c2, float grow, int lane) {
+__device__ __forceinline__ void fwd_scores(const char* Ks, const Chunk (&qf)[Frag<T, D>::KK], f32x16 (&s)[NB], int lane) {
   constexpr int KK = Frag<T, D>::KK, RB = Frag<T, D>::RB;
   const int hf = lane >> 5, c = lane & 31;
-  f32x16 s[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     s[nb] = f32x16{};
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) mfma_step<T>(lds_chunk<RB>(Ks, nb * 32 + c, 2 * kk + hf), qf[kk], s[nb]);
   }
+}
+
+// Masks a tile's scores and moves the row's reference m (of the weights exp(scale (s - m))) where it has to; returns
+// the exponent's offset.
+template <int D, int NB>
+__device__ __forceinline__ float fwd_reference(f32x16 (&s)[NB], f32x16 (&o)[D / 32], float& m, float& l, int key0, int lim, float c2,
+                                               float grow, int hf) {
   if (!__all(key0 + NB * 32 - 1 <= lim)) {
     rare_branch();
 #pragma unroll
@@ -44,9 +52,9 @@ __device__ __forceinline__ void fwd_tile(const char* Ks, const char* Vs, const C
 #pragma unroll
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[nb][i]);
   mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-  // The reference of the weights moves only where a row's maximum passed it by more than 2^8 (in weight): until
-  // then weights up to 2^8 are as exact in fp32 and bf16 as those up to 1, and O need not be rescaled.  Each row
-  // decides for itself, so its result does not depend on the rows beside it.
+  // The reference moves only where a row's maximum passed it by more than 2^8 (in weight): until then weights up to
+  // 2^8 are as exact in fp32 and bf16 as those up to 1, and O need not be rescaled.  Each row decides for itself, so
+  // its result does not depend on the rows beside it.
   if (__any(mx > m + grow)) {
     rare_branch();
     const float mn = mx > m + grow ? mx : m, mz = mn == -INFINITY ? 0.f : mn;
@@ -59,7 +67,7 @@ __device__ __forceinline__ void fwd_tile(const char* Ks, const char* Vs, const C
       for (int i = 0; i < 16; ++i) o[db][i] *= corr;
   }
   const float mz = m == -INFINITY ? 0.f : m;   // nothing visible yet: every weight is exp2(-inf) = 0
-  float mu = mz * c2;
+  const float mu = mz * c2;
   // exp2(s * c2 - mu) in one fma: mu's rounding is the same factor in every weight of the row and cancels, unless
   // it is large itself; then the reference is subtracted first
   if (__any(fabsf(mu) > 16777216.f)) {
@@ -68,8 +76,12 @@ __device__ __forceinline__ void fwd_tile(const char* Ks, const char* Vs, const C
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[nb][i] -= mz;
-    mu = 0.f;
+    return 0.f;
   }
+  return mu;
+}
+
+template <int NB> __device__ __forceinline__ void fwd_weights(f32x16 (&s)[NB], float& l, float c2, float mu) {
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -78,8 +90,6 @@ __device__ __forceinline__ void fwd_tile(const char* Ks, const char* Vs, const C
       s[nb][i] = p;
       l += p;
     }
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) accum_xt<T, D>(Vs, nb * 32, s[nb], o, lane);
 }
 
 // One row tile over keys kt0 * BN .. of its sequence.
@@ -110,12 +120,15 @@ __device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* tiles, int h
   TileCopy<T, D, BN, NW> kc, vc;
   kc.init(wave, lane, a.D, a.rk);
   vc.init(wave, lane, a.D, a.rv);
-  // K and V tiles, two of each: the next is under way while one is used
-  auto stage = [&](int kt, int at) {
-    kc.load(kb + (long)kt * BN * a.rk, a.rk, lk - kt * BN, tiles + at, wave, lane, a.D);
-    vc.load(vb + (long)kt * BN * a.rv, a.rv, lk - kt * BN, tiles + at + TB, wave, lane, a.D);
-  };
-  if (kt0 < kt1) stage(kt0, 0);
+  // two K and two V tiles: while tile kt's weights are formed, tile kt + 1's scores are (its K is there) and K of
+  // kt + 2 and V of kt + 1 are under way
+  auto stage_k = [&](int kt, int at) { kc.load(kb + (long)kt * BN * a.rk, a.rk, lk - kt * BN, tiles + at, wave, lane, a.D); };
+  auto stage_v = [&](int kt, int at) { vc.load(vb + (long)kt * BN * a.rv, a.rv, lk - kt * BN, tiles + 2 * TB + at, wave, lane, a.D); };
+  if (kt0 < kt1) {
+    stage_k(kt0, 0);
+    stage_v(kt0, 0);
+    if (kt0 + 1 < kt1) stage_k(kt0 + 1, TB);
+  }
 
   const int r = r0 + wave * 32 + c, pos = group_div(r, a.G, a.gmagic), hg = r - pos * a.G;
   const bool live = r < rows;
@@ -136,10 +149,31 @@ __device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* tiles, int h
   float m = -INFINITY, l = 0.f;   // m: of q . k, before the scale; l: this lane's half of the row
   const float c2 = a.scale * LOG2E, grow = 8.f / c2;
 
-  for (int kt = kt0, at = 0; kt < kt1; ++kt, at ^= 2 * TB) {
+  if (kt0 < kt1) {
+    f32x16 s[NB];
     tiles_ready();
-    if (kt + 1 < kt1) stage(kt + 1, at ^ (2 * TB));
-    fwd_tile<T, D, NB>(tiles + at, tiles + at + TB, qf, o, m, l, kt * BN, lim, c2, grow, lane);
+    fwd_scores<T, D, NB>(tiles, qf, s, lane);
+    int at = 0;
+    for (int kt = kt0; kt + 1 < kt1; ++kt, at ^= TB) {
+      const float mu = fwd_reference<D, NB>(s, o, m, l, kt * BN, lim, c2, grow, hf);
+      tiles_ready();   // K of kt + 1, V of kt; and everybody is done with K of kt and V of kt - 1
+      if (kt + 2 < kt1) stage_k(kt + 2, at);
+      stage_v(kt + 1, at ^ TB);
+      // the next scores' matrix instructions run under this tile's exponentials
+      f32x16 next[NB];
+      fwd_scores<T, D, NB>(tiles + (at ^ TB), qf, next, lane);
+      fwd_weights<NB>(s, l, c2, mu);
+      OGV_INTERLEAVE
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) accum_xt<T, D>(tiles + 2 * TB + at, nb * 32, s[nb], o, lane);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) s[nb] = next[nb];
+    }
+    const float mu = fwd_reference<D, NB>(s, o, m, l, (kt1 - 1) * BN, lim, c2, grow, hf);
+    tiles_ready();
+    fwd_weights<NB>(s, l, c2, mu);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) accum_xt<T, D>(tiles + 2 * TB + at, nb * 32, s[nb], o, lane);
   }
 
   l += __shfl_xor(l, 32, 64);
