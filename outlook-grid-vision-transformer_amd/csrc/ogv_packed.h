@@ -92,6 +92,24 @@ union Chunk {
   f32x4 f;
 };
 
+// a: this lane's of lanes 0..31 and its partner's (lane ^ 32) of lanes 32..63 afterwards stand where the MFMA layout
+// has halves apart: (a, b) -> ({a of the lower half, b of the lower half}, {a of the upper half, b of the upper half})
+__device__ __forceinline__ void swap_halves(unsigned& a, unsigned& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0], b = r[1];
+}
+// the larger of a value and its partner's in lane ^ 32
+__device__ __forceinline__ float pair_max(float v) {
+  unsigned a = __builtin_bit_cast(unsigned, v), b = a;
+  swap_halves(a, b);
+  return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+  unsigned a = __builtin_bit_cast(unsigned, v), b = a;
+  swap_halves(a, b);
+  return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+
 __device__ __forceinline__ Chunk zero_chunk() {
   Chunk c;
   c.u = make_uint4(0, 0, 0, 0);
@@ -213,6 +231,37 @@ __device__ __forceinline__ void accum_xt(const char* tile, int row0, const f32x1
         acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, y[i], acc[db], 0, 0, 0);
       }
     }
+  }
+}
+
+// Store a C tile (column c is an output row, registers its dims) times mul at p, the lane's output row.  Lanes c and
+// c + 32 hold alternate groups of 4 dims; bf16 rows trade groups, so that a lane writes 16 bytes at once.  Every lane
+// of the wave comes here; `live` says whether its row is written.
+template <typename T, int D>
+__device__ __forceinline__ void store_cols(T* p, const f32x16 (&x)[D / 32], float mul, int Dlive, int hf, bool live) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; g += 2) {
+        union { bf16 h[4]; unsigned u[2]; } lo, hi;   // dims 8 * g + 4 * hf .. and 8 * (g + 1) + 4 * hf ..
+#pragma unroll
+        for (int e = 0; e < 4; ++e) lo.h[e] = (bf16)(x[db][4 * g + e] * mul), hi.h[e] = (bf16)(x[db][4 * g + 4 + e] * mul);
+        swap_halves(lo.u[0], hi.u[0]);
+        swap_halves(lo.u[1], hi.u[1]);
+        const int d = db * 32 + 8 * (g + hf);
+        if (live && d < Dlive) *reinterpret_cast<uint4*>(p + d) = make_uint4(lo.u[0], lo.u[1], hi.u[0], hi.u[1]);
+      }
+  } else {
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = db * 32 + 8 * g + 4 * hf;
+        if (live && d < Dlive)
+          *reinterpret_cast<float4*>(p + d) = make_float4(x[db][4 * g] * mul, x[db][4 * g + 1] * mul, x[db][4 * g + 2] * mul,
+                                                          x[db][4 * g + 3] * mul);
+      }
   }
 }
 

@@ -20,21 +20,6 @@ bool aligned16(std::initializer_list<const void*> ps);
 
 constexpr float BLOG2E = 1.4426950408889634f;
 
-// Store a 32-column C tile block (columns c, dims 32 * db + rows) times mul as rows of the output.
-template <typename T, int D>
-__device__ __forceinline__ void store_cols(T* p, const f32x16 (&x)[D / 32], float mul, int Dlive, int hf) {
-#pragma unroll
-  for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = db * 32 + 8 * g + 4 * hf;
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = x[db][4 * g + e] * mul;
-      if (d < Dlive) store_vec<T, 4>(p + d, v);
-    }
-}
-
 // 32 * NB keys of dq: scores and dp transposed (columns are rows r), dQ^T += K^T dS^T
 template <typename T, int D, int NB>
 __device__ __forceinline__ void dq_tile(const char* Ks, const char* Vs, const Chunk (&qf)[Frag<T, D>::KK],
@@ -123,7 +108,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dq_ker
       }
     }
   }
-  delta += __shfl_xor(delta, 32, 64);
+  delta = pair_sum(delta);
   // a row that sees nothing has lse = -inf: +inf keeps its weights at exp2(-inf) = 0
   float lse2 = live ? a.lse[orow] * BLOG2E : INFINITY;
   if (lse2 == -INFINITY) lse2 = INFINITY;
@@ -139,8 +124,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dq_ker
     dq_tile<T, D, NB>(tiles + at, tiles + at + TB, qf, gf, dq, kt * BN, lim, c2, lse2, delta, lane);
   }
 
-  if (r >= store_rows) return;
-  store_cols<T, D>((T*)a.dq + (long)(sq.start + pos) * a.rdq + (long)(h * a.G + hg) * a.hsdq, dq, a.scale, a.D, hf);
+  store_cols<T, D>((T*)a.dq + (long)(sq.start + pos) * a.rdq + (long)(h * a.G + hg) * a.hsdq, dq, a.scale, a.D, hf, r < store_rows);
 }
 
 // 32 * NB rows of dk / dv: scores and dp with columns = keys, dV^T += dO^T P, dK^T += Q^T dS
@@ -292,19 +276,19 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dkv_ke
     dkv_tile<T, D, NB, VL>(tiles + at, tiles + at + TB, S, kf, vf, Vw, dk, dv, rt, off, j, jmax, a, c2, lane);
   }
 
-  if (j >= store_keys) return;
+  const bool out = j < store_keys;
   if (!live) {   // keys behind the last sequence
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) dk[db] = f32x16{}, dv[db] = f32x16{};
   }
   if (a.nsplit > 1) {
     const long n = (long)a.Mk * a.hkv, row = (long)(sk.start + j) * a.hkv + h;
-    store_cols<float, D>(a.part_o + ((2L * split) * n + row) * a.D, dk, 1.f, a.D, hf);
-    store_cols<float, D>(a.part_o + ((2L * split + 1) * n + row) * a.D, dv, 1.f, a.D, hf);
+    store_cols<float, D>(a.part_o + ((2L * split) * n + row) * a.D, dk, 1.f, a.D, hf, out);
+    store_cols<float, D>(a.part_o + ((2L * split + 1) * n + row) * a.D, dv, 1.f, a.D, hf, out);
     return;
   }
-  store_cols<T, D>((T*)a.dk + (long)(sk.start + j) * a.rdk + (long)h * a.hsdk, dk, a.scale, a.D, hf);
-  store_cols<T, D>((T*)a.dv + (long)(sk.start + j) * a.rdv + (long)h * a.hsdv, dv, 1.f, a.D, hf);
+  store_cols<T, D>((T*)a.dk + (long)(sk.start + j) * a.rdk + (long)h * a.hsdk, dk, a.scale, a.D, hf, out);
+  store_cols<T, D>((T*)a.dv + (long)(sk.start + j) * a.rdv + (long)h * a.hsdv, dv, 1.f, a.D, hf, out);
 }
 
 // dk, dv = sums of the row pieces, in order

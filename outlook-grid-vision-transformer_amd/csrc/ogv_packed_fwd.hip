@@ -15,9 +15,6 @@
 
 namespace ogv {
 
-#ifndef OGV_INTERLEAVE
-#define OGV_INTERLEAVE
-#endif
 constexpr float LOG2E = 1.4426950408889634f;
 
 // S^T = K Q^T of one key tile.
@@ -51,7 +48,7 @@ __device__ __forceinline__ float fwd_reference(f32x16 (&s)[NB], f32x16 (&o)[D / 
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[nb][i]);
-  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+  mx = pair_max(mx);
   // The reference moves only where a row's maximum passed it by more than 2^8 (in weight): until then weights up to
   // 2^8 are as exact in fp32 and bf16 as those up to 1, and O need not be rescaled.  Each row decides for itself, so
   // its result does not depend on the rows beside it.
@@ -163,7 +160,6 @@ __device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* tiles, int h
       f32x16 next[NB];
       fwd_scores<T, D, NB>(tiles + (at ^ TB), qf, next, lane);
       fwd_weights<NB>(s, l, c2, mu);
-      OGV_INTERLEAVE
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) accum_xt<T, D>(tiles + 2 * TB + at, nb * 32, s[nb], o, lane);
 #pragma unroll
@@ -176,38 +172,21 @@ __device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* tiles, int h
     for (int nb = 0; nb < NB; ++nb) accum_xt<T, D>(tiles + 2 * TB + at, nb * 32, s[nb], o, lane);
   }
 
-  l += __shfl_xor(l, 32, 64);
-  if (r >= store_rows) return;
+  l = pair_sum(l);
+  const bool out = r < store_rows;
   const long orow = (long)(start + pos) * a.hq + h * a.G + hg;   // row of the [Mq * hq] outputs
   if (SPLIT) {   // unnormalised partials, joined by packed_join_kernel
     const long at = (long)piece * a.Mq * a.hq + orow;
-    float* po = a.part_o + at * a.D;
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int d = db * 32 + 8 * g + 4 * hf;
-        if (d < a.D) *reinterpret_cast<float4*>(po + d) = make_float4(o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]);
-      }
-    if (hf == 0) {
+    store_cols<float, D>(a.part_o + at * a.D, o, 1.f, a.D, hf, out);
+    if (out && hf == 0) {
       *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(m, l);
       if (piece == 0) a.part_n[orow] = pieces;
     }
     return;
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);   // (NaN stays NaN)
-  T* op = (T*)a.out + (long)(start + pos) * a.ro + (long)(h * a.G + hg) * a.hso;
-#pragma unroll
-  for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = db * 32 + 8 * g + 4 * hf;
-      float x[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = o[db][4 * g + e] * inv;
-      if (d < a.D) store_vec<T, 4>(op + d, x);
-    }
-  if (hf == 0) a.lse[orow] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+  store_cols<T, D>((T*)a.out + (long)(start + pos) * a.ro + (long)(h * a.G + hg) * a.hso, o, inv, a.D, hf, out);
+  if (out && hf == 0) a.lse[orow] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
 }
 
 template <typename T, int D, int NW, bool SPLIT>
@@ -230,32 +209,38 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_fwd_ke
   }
 }
 
-// out = sum_s w_s o_s / sum_s w_s l_s, w_s = exp(scale (m_s - max m)), over a row's key pieces in order
+// out = sum_s w_s o_s / sum_s w_s l_s, w_s = exp(scale (m_s - max m)), over a row's key pieces in order.  A wave joins
+// a row: lane s holds piece s's weight (at most 64), then the lanes are the dims.
 template <typename T>
 __global__ __launch_bounds__(256) void packed_join_kernel(const PackedArgs a) {
-  const int per = a.D / 4;
-  const long n = (long)a.Mq * a.hq * per, idx = (long)blockIdx.x * 256 + threadIdx.x;
-  if (idx >= n) return;
-  const long row = idx / per, R = (long)a.Mq * a.hq;
-  const int d = (int)(idx - row * per) * 4, pieces = a.part_n[row];
-  float m = -INFINITY;
-  for (int s = 0; s < pieces; ++s) m = fmaxf(m, a.part_ml[2 * (s * R + row)]);
-  const float mu = m == -INFINITY ? 0.f : m, c2 = a.scale * LOG2E;
-  float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = 0; s < pieces; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (s * R + row));
-    const float4 p = *reinterpret_cast<const float4*>(a.part_o + (s * R + row) * a.D + d);
-    const float w = __builtin_amdgcn_exp2f((ml.x - mu) * c2);
-    l += w * ml.y;
-    x[0] += w * p.x, x[1] += w * p.y, x[2] += w * p.z, x[3] += w * p.w;
-  }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const int lane = threadIdx.x & 63;
+  const long R = (long)a.Mq * a.hq, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= R) return;
+  const int pieces = __builtin_amdgcn_readfirstlane(a.part_n[row]);
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < a.nsplit) ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (lane * R + row));
+  if (lane >= pieces) ml = make_float2(-INFINITY, 0.f);   // (never written)
+  const float m = group_max<64>(ml.x), mu = m == -INFINITY ? 0.f : m;
+  float w = __builtin_amdgcn_exp2f((ml.x - mu) * (a.scale * LOG2E));
+  const float l = wave_sum(w * ml.y);
+  w *= l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);   // (NaN stays NaN)
+  const int d = 2 * lane;
+  float x = 0.f, y = 0.f;
+  const float* po = a.part_o + row * a.D + (d < a.D ? d : 0);
+  for (int s = 0; s < pieces; s += 4) {   // four loads under way; past the last piece it is repeated with weight 0
+    float2 p[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] *= inv;
+    for (int u = 0; u < 4; ++u) p[u] = *reinterpret_cast<const float2*>(po + min(s + u, pieces - 1) * R * a.D);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float ws = s + u < pieces ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s + u)) : 0.f;
+      x = fmaf(ws, p[u].x, x), y = fmaf(ws, p[u].y, y);
+    }
+  }
   const long q = row / a.hq;
-  store_vec<T, 4>((T*)a.out + q * a.ro + (row - q * a.hq) * a.hso + d, x);
-  if (d == 0) a.lse[row] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+  const float v[2] = {x, y};
+  if (d < a.D) store_vec<T, 2>((T*)a.out + q * a.ro + (row - q * a.hq) * a.hso + d, v);
+  if (lane == 0) a.lse[row] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
 }
 
 struct FwdPlan {
@@ -288,7 +273,7 @@ static void fwd_launch(const FwdPlan& p, const PackedArgs& a, hipStream_t s) {
   if (p.nsplit > 1) {
     if (p.nw == 4) packed_fwd_kernel<T, D, 4, true><<<p.grid, 256, 0, s>>>(a);
     else packed_fwd_kernel<T, D, 1, true><<<p.grid, 64, 0, s>>>(a);
-    packed_join_kernel<T><<<cdiv((long)a.Mq * a.hq * (a.D / 4), 256), 256, 0, s>>>(a);
+    packed_join_kernel<T><<<cdiv((long)a.Mq * a.hq, 4), 256, 0, s>>>(a);
   } else {
     if (p.nw == 4) packed_fwd_kernel<T, D, 4, false><<<p.grid, 256, 0, s>>>(a);
     else packed_fwd_kernel<T, D, 1, false><<<p.grid, 64, 0, s>>>(a);
