@@ -11,8 +11,8 @@
 //
 // Bound by memory: forward f, x -> y, h (4 rows of C), backward f, x, dy, dh -> df, dx (6).  A row belongs to
 // G lanes (a part of a wave, a wave, or a workgroup) that keep it in registers through every reduction.
-// Column sums: each lane adds its columns over the workgroup's rows, one partial row per workgroup, then the
-// fixed-order column reduction: no atomics.
+// Column sums: each lane adds its columns over the workgroup's rows, one partial row per workgroup, then they are added
+// in a fixed order: no atomics.
 #include "ogv_common.h"
 
 #include <initializer_list>
@@ -26,7 +26,7 @@ struct GnArgs {
   void *y, *h, *df, *dx;
   const float *gate, *rs, *w0, *b0, *w1, *b1;   // 0: post, 1: pre
   float* stats;     // [M][4]: post mean, post rstd, pre mean, pre rstd
-  float *part, *gpart;   // backward column sums: [blocks][4 or 5][C]; per-sample gate: [units][C]
+  float *part, *gpart;   // backward column sums: [blocks][4][C]; per-sample gate: [units][C]
   long M;
   int C, k0, k1, rps;
   int S, nch;       // gate samples (1: the gate has no samples), row chunks per sample
@@ -179,62 +179,91 @@ __device__ __forceinline__ void flush_sums(float (&s)[NV * VEC], float* __restri
   for (int e = 0; e < E; ++e) s[e] = 0.f;
 }
 
-template <typename T, int G, int NV, int VEC>
+// The raw values of a row that the backward reads, loaded one row ahead of their use.
+template <typename T, int G, int NV, int VEC> struct BackRow {
+  RawVec<T, VEC> f[NV], x[NV], dy[NV], dh[NV];
+  float4 st;
+  float rs;
+  __device__ __forceinline__ void load(const GnArgs& a, long row, int lg) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * G + lg) * VEC;
+      const long at = row * a.C + (c < a.C ? c : 0);
+      f[v].load((const T*)a.f + at);
+      x[v].load((const T*)a.x + at);
+      if (a.dy) dy[v].load((const T*)a.dy + at);
+      if (a.dh) dh[v].load((const T*)a.dh + at);
+    }
+    st = *reinterpret_cast<const float4*>(a.stats + row * 4);
+    rs = a.rs ? a.rs[row / a.rps] : 1.f;
+  }
+};
+
+// Column sums kept per lane: A = sum s_b dY fhat and B = sum s_b dY (fhat = f without a post norm) give every gradient
+// of the branch's side -- dgate = w A + b B, dw = gate A, db = gate B -- so a gate per channel needs no third sum, and a
+// gate per sample (SMP) closes A and B into s0, t0 at a sample's end.  s1, t1: the pre norm's.
+template <typename T, int G, int NV, int VEC, bool SMP>
 __global__ __launch_bounds__(256) void gated_norm_bwd_kernel(const GnArgs a) {
   constexpr int E = NV * VEC, R = 256 / G, L = G < 64 ? G : 64;
   __shared__ float red[4];
   __shared__ float buf[G < 256 ? 4 * E * L : 1];
   const int lg = threadIdx.x % G, C = a.C;
   const float invC = 1.f / (float)C;
-  bool in[E];
+  bool in[NV];
   float gw[E], w0[E], b0[E], w1[E];
-  float sg[E], s0[E], t0[E], s1[E], t1[E];   // dgate, dw0, db0, dw1, db1
+  float A[E], B[E], s1[E], t1[E], s0[SMP ? E : 1], t0[SMP ? E : 1];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) in[v] = (v * G + lg) * VEC < C;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int c = ((e / VEC) * G + lg) * VEC + e % VEC, cc = c < C ? c : 0;
-    in[e] = c < C;
-    gw[e] = a.gate && a.S == 1 ? a.gate[cc] : 1.f;
+    gw[e] = a.gate && !SMP ? a.gate[cc] : 1.f;
     w0[e] = a.w0 ? a.w0[cc] : 1.f;
     b0[e] = a.b0 ? a.b0[cc] : 0.f;
     w1[e] = a.w1 ? a.w1[cc] : 1.f;
-    sg[e] = s0[e] = t0[e] = s1[e] = t1[e] = 0.f;
+    A[e] = B[e] = s1[e] = t1[e] = 0.f;
+    if constexpr (SMP) s0[e] = t0[e] = 0.f;
   }
   const long units = (long)a.S * a.nch;
   for (long u = blockIdx.x; u < units; u += gridDim.x) {
     const long smp = u / a.nch, ch = u - smp * a.nch;
     const long beg = smp * a.rows_s + ch * a.rows_c, end = min(beg + a.rows_c, (smp + 1) * a.rows_s);
-    if (a.S > 1) {
+    if constexpr (SMP) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int c = ((e / VEC) * G + lg) * VEC + e % VEC;
         gw[e] = a.gate[smp * C + (c < C ? c : 0)];
       }
     }
-    for (long row = beg + threadIdx.x / G; row < end; row += R) {
-      float f[E], x[E], dy[E], dh[E];
-      const float4 st = *reinterpret_cast<const float4*>(a.stats + row * 4);
+    long row = beg + threadIdx.x / G;
+    BackRow<T, G, NV, VEC> next;
+    if (row < end) next.load(a, row, lg);
+    for (; row < end; row += R) {
+      float f[E], x[E], dY[E];
+      const float4 st = next.st;
+      const float rs = next.rs;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int c = (v * G + lg) * VEC, cc = c < C ? c : 0;
-        load_vec<T, VEC>((const T*)a.f + row * C + cc, f + v * VEC);
-        load_vec<T, VEC>((const T*)a.x + row * C + cc, x + v * VEC);
-        if (a.dy) load_vec<T, VEC>((const T*)a.dy + row * C + cc, dy + v * VEC);
-        if (a.dh) load_vec<T, VEC>((const T*)a.dh + row * C + cc, dh + v * VEC);
+        next.f[v].unpack(f + v * VEC);
+        next.x[v].unpack(x + v * VEC);
       }
-      const float rs = a.rs ? a.rs[row / a.rps] : 1.f;
-      float n[E], dY[E];
+      float dh[E], dy[E];
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        if (a.dy) next.dy[v].unpack(dy + v * VEC);
+        if (a.dh) next.dh[v].unpack(dh + v * VEC);
+      }
+      next.load(a, min(row + R, end - 1), lg);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        f[e] = in[e] ? f[e] : 0.f;
-        if (a.k0 != NK_NONE) f[e] = in[e] ? (f[e] - st.x) * st.y : 0.f;
-        n[e] = a.k0 != NK_NONE ? fmaf(f[e], w0[e], b0[e]) : f[e];
+        f[e] = in[e / VEC] ? (a.k0 != NK_NONE ? (f[e] - st.x) * st.y : f[e]) : 0.f;   // fhat
         dY[e] = 0.f;
       }
       if (a.dh) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          x[e] = in[e] ? (fmaf(rs * gw[e], n[e], a.alpha * x[e]) - st.z) * st.w : 0.f;   // yhat
-          const float g = in[e] ? dh[e] : 0.f;
+          x[e] = in[e / VEC] ? (fmaf(rs * gw[e], fmaf(f[e], w0[e], b0[e]), a.alpha * x[e]) - st.z) * st.w : 0.f;   // yhat
+          const float g = in[e / VEC] ? dh[e] : 0.f;
           s1[e] = fmaf(g, x[e], s1[e]);
           t1[e] += g;
           dY[e] = g * w1[e];
@@ -243,46 +272,87 @@ __global__ __launch_bounds__(256) void gated_norm_bwd_kernel(const GnArgs a) {
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        if (a.dy) dY[e] += in[e] ? dy[e] : 0.f;
+        if (a.dy) dY[e] += in[e / VEC] ? dy[e] : 0.f;
         x[e] = a.alpha * dY[e];
-        sg[e] = fmaf(rs * n[e], dY[e], sg[e]);
-        dY[e] *= rs * gw[e];   // dn
+        dY[e] *= rs;
+        A[e] = fmaf(dY[e], f[e], A[e]);
+        B[e] += dY[e];
+        dY[e] *= gw[e];   // dn
       }
 #pragma unroll
       for (int v = 0; v < NV; ++v)
-        if (in[v * VEC]) store_vec<T, VEC>((T*)a.dx + row * C + (v * G + lg) * VEC, x + v * VEC);
+        if (in[v]) store_vec<T, VEC>((T*)a.dx + row * C + (v * G + lg) * VEC, x + v * VEC);
       if (a.k0 != NK_NONE) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          s0[e] = fmaf(dY[e], f[e], s0[e]);
-          t0[e] += dY[e];
-          dY[e] *= in[e] ? w0[e] : 0.f;
-        }
+        for (int e = 0; e < E; ++e) dY[e] *= in[e / VEC] ? w0[e] : 0.f;
         norm_back<G, E>(dY, f, a.k0, invC, st.y, red);
       }
 #pragma unroll
       for (int v = 0; v < NV; ++v)
-        if (in[v * VEC]) store_vec<T, VEC>((T*)a.df + row * C + (v * G + lg) * VEC, dY + v * VEC);
+        if (in[v]) store_vec<T, VEC>((T*)a.df + row * C + (v * G + lg) * VEC, dY + v * VEC);
     }
-    if (a.S > 1) flush_sums<G, NV, VEC>(sg, a.gpart + u * C, C, buf);
+    if constexpr (SMP) {
+      float d[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        d[e] = fmaf(w0[e], A[e], b0[e] * B[e]);
+        s0[e] = fmaf(gw[e], A[e], s0[e]);
+        t0[e] = fmaf(gw[e], B[e], t0[e]);
+        A[e] = B[e] = 0.f;
+      }
+      flush_sums<G, NV, VEC>(d, a.gpart + u * C, C, buf);
+    }
   }
-  float* out = a.part + (long)blockIdx.x * 5 * C;
-  flush_sums<G, NV, VEC>(sg, out, C, buf);
-  flush_sums<G, NV, VEC>(s1, out + C, C, buf);
-  flush_sums<G, NV, VEC>(t1, out + 2 * C, C, buf);
-  flush_sums<G, NV, VEC>(s0, out + 3 * C, C, buf);
-  flush_sums<G, NV, VEC>(t0, out + 4 * C, C, buf);
+  float* out = a.part + (long)blockIdx.x * 4 * C;
+  if constexpr (SMP) {
+    flush_sums<G, NV, VEC>(s0, out, C, buf);
+    flush_sums<G, NV, VEC>(t0, out + C, C, buf);
+  } else {
+    flush_sums<G, NV, VEC>(A, out, C, buf);
+    flush_sums<G, NV, VEC>(B, out + C, C, buf);
+  }
+  flush_sums<G, NV, VEC>(s1, out + 2 * C, C, buf);
+  flush_sums<G, NV, VEC>(t1, out + 3 * C, C, buf);
 }
 
-// dgate[s][c] = sum of the sample's row chunks, in order
-__global__ __launch_bounds__(256) void gate_sum_kernel(const float* __restrict__ gpart, float* __restrict__ dgate, long n,
-                                                       int C, int nch) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const long s = i / C, c = i - s * C;
-  float v = 0.f;
-  for (int j = 0; j < nch; ++j) v += gpart[(s * nch + j) * C + c];
-  dgate[i] = v;
+// The partial rows part [rows][4][C] added in a fixed order into sums [5][C] = dgate, d pre_w, d pre_b, d post_w, d post_b,
+// and dgate [S][C] from the samples' row chunks.  Workgroup: 64 columns of one pair of sums, 16 waves on every 16th row.
+__global__ __launch_bounds__(1024) void gated_norm_sum_kernel(const GnArgs a, float* __restrict__ sums, float* __restrict__ dgate,
+                                                              int rows, int colblocks) {
+  const int C = a.C, bx = blockIdx.x;
+  if (bx >= 2 * colblocks) {
+    const long i = (long)(bx - 2 * colblocks) * 1024 + threadIdx.x;
+    if (i >= (long)a.S * C) return;
+    const long s = i / C, c = i - s * C;
+    float v = 0.f;
+    for (int j = 0; j < a.nch; ++j) v += a.gpart[(s * a.nch + j) * C + c];
+    dgate[i] = v;
+    return;
+  }
+  __shared__ float red[2][16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pair = bx / colblocks;
+  const int c = (bx - pair * colblocks) * 64 + lane, cc = min(c, C - 1);
+  const float* p = a.part + 2L * pair * C + cc;
+  float x = 0.f, y = 0.f;
+#pragma unroll 8
+  for (int r = wave; r < rows; r += 16) {
+    x += p[(long)r * 4 * C];
+    y += p[(long)r * 4 * C + C];
+  }
+  red[0][wave][lane] = x, red[1][wave][lane] = y;
+  __syncthreads();
+  if (wave || c >= C) return;
+  x = y = 0.f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) x += red[0][w][lane], y += red[1][w][lane];
+  if (pair) {
+    sums[C + c] = x, sums[2 * C + c] = y;
+  } else if (a.S > 1) {
+    sums[3 * C + c] = x, sums[4 * C + c] = y;
+  } else {
+    const float g = a.gate ? a.gate[c] : 1.f, w = a.w0 ? a.w0[c] : 1.f, b = a.b0 ? a.b0[c] : 0.f;
+    sums[c] = fmaf(w, x, b * y), sums[3 * C + c] = g * x, sums[4 * C + c] = g * y;
+  }
 }
 
 // Lanes per row and columns per lane: vectors where the channel count and the pointers allow them; up to 1024
@@ -308,7 +378,7 @@ static bool gn_plan(int C, bool vec, GnPlan& p) {
   }
   p.G = n <= 512 ? 64 : 256;
   p.NV = (n + p.G - 1) / p.G;
-  for (int nv : {1, 2, 4, 8, 16, 32})
+  for (int nv : {1, 2, 4, 6, 8, 16, 32})
     if (p.NV <= nv) {
       p.NV = nv;
       return true;
@@ -316,7 +386,7 @@ static bool gn_plan(int C, bool vec, GnPlan& p) {
   return false;
 }
 
-constexpr long GN_BLOCKS = 1024;   // partial rows of the backward's column sums
+constexpr long GN_BLOCKS = 512;   // workgroups of the backward (two to a CU), and partial rows of its column sums
 
 static void gn_units(long M, long samples, const GnPlan& p, GnArgs& a, long& blocks) {
   a.S = (int)samples;
@@ -333,7 +403,8 @@ static void gn_units(long M, long samples, const GnPlan& p, GnArgs& a, long& blo
 
 template <typename T, int G, int NV, int VEC>
 static void gn_run(const GnArgs& a, bool bwd, long blocks, hipStream_t s) {
-  if (bwd) gated_norm_bwd_kernel<T, G, NV, VEC><<<(unsigned)blocks, 256, 0, s>>>(a);
+  if (bwd && a.S > 1) gated_norm_bwd_kernel<T, G, NV, VEC, true><<<(unsigned)blocks, 256, 0, s>>>(a);
+  else if (bwd) gated_norm_bwd_kernel<T, G, NV, VEC, false><<<(unsigned)blocks, 256, 0, s>>>(a);
   else gated_norm_fwd_kernel<T, G, NV, VEC><<<(unsigned)blocks, 256, 0, s>>>(a);
 }
 
@@ -359,10 +430,11 @@ template <typename T> static void gn_dispatch(const GnPlan& p, const GnArgs& a, 
     if (p.NV == 1) return gn_run<T, 64, 1, 1>(a, bwd, blocks, s);
     if (p.NV == 2) return gn_run<T, 64, 2, 1>(a, bwd, blocks, s);
     if (p.NV == 4) return gn_run<T, 64, 4, 1>(a, bwd, blocks, s);
+    if (p.NV == 6) return gn_run<T, 64, 6, 1>(a, bwd, blocks, s);
     return gn_run<T, 64, 8, 1>(a, bwd, blocks, s);
   }
   if (p.NV <= 4) return gn_run<T, 256, 4, 1>(a, bwd, blocks, s);
-  if (p.NV == 8) return gn_run<T, 256, 8, 1>(a, bwd, blocks, s);
+  if (p.NV <= 8) return gn_run<T, 256, 8, 1>(a, bwd, blocks, s);
   if (p.NV == 16) return gn_run<T, 256, 16, 1>(a, bwd, blocks, s);
   return gn_run<T, 256, 32, 1>(a, bwd, blocks, s);
 }
@@ -422,8 +494,7 @@ extern "C" size_t ogv_gated_norm_bwd_ws_bytes(const ogv_gated_norm_desc* d, ogv_
     if (!gn_plan(d->C, vec, p)) continue;
     for (long samples : {1L, (long)d->samples}) {   // (nor whether there is a gate)
       gn_units(d->M, samples, p, a, blocks);
-      const size_t n = (size_t)blocks * 5 * d->C + colreduce_tmp_floats(blocks, 5L * d->C) +
-                       (a.S > 1 ? (size_t)a.S * a.nch * d->C : 0);
+      const size_t n = (size_t)blocks * 4 * d->C + (a.S > 1 ? (size_t)a.S * a.nch * d->C : 0);
       if (n > most) most = n;
     }
   }
@@ -447,15 +518,11 @@ extern "C" int ogv_gated_norm_bwd(const void* dy, const void* dh, const void* f,
   long blocks;
   gn_units(d->M, gate ? d->samples : 1, p, a, blocks);
   a.part = (float*)ws;
-  float* tmp = a.part + (size_t)blocks * 5 * d->C;
-  a.gpart = tmp + colreduce_tmp_floats(blocks, 5L * d->C);
+  a.gpart = a.part + (size_t)blocks * 4 * d->C;
   hipStream_t s = as_stream(stream);
   if (dt == OGV_BF16) gn_dispatch<bf16>(p, a, true, blocks, s);
   else gn_dispatch<float>(p, a, true, blocks, s);
-  colreduce(a.part, sums, blocks, 5L * d->C, 5L * d->C, tmp, s);
-  if (a.S > 1) {
-    const long n = (long)a.S * d->C;
-    gate_sum_kernel<<<cdiv(n, 256), 256, 0, s>>>(a.gpart, dgate, n, d->C, a.nch);
-  }
+  const int cb = (int)cdiv(d->C, 64);
+  gated_norm_sum_kernel<<<2 * cb + (a.S > 1 ? cdiv((long)a.S * d->C, 1024) : 0), 1024, 0, s>>>(a, sums, dgate, (int)blocks, cb);
   return check_launch("ogv_gated_norm_bwd");
 }
