@@ -317,17 +317,18 @@ struct BwdPlan {
 };
 
 // Waves per workgroup as in the forward.  The rows of dk / dv are split while the key tiles would not fill the 256 CUs
-// three times (under the causal mask the first tile has twice the average work), at least 512 rows to a piece: a piece
-// costs 16 bytes of partial sums per key, head and dim.
-static BwdPlan bwd_plan(const ogv_packed_desc* d) {
+// twice, into 1024 workgroups or a few more (two to a CU, twice: under the causal mask the first tile has twice the
+// average work; long causal streams, D = 128: 580 us for the step with 768, 549 with 1024, 569 with 1536).  A piece costs 16 bytes of partial sums
+// per key, head and dim, so it has at least 512 rows on average, 32 in fp32, whose products run at a sixteenth of the rate.
+static BwdPlan bwd_plan(const ogv_packed_desc* d, ogv_dtype dt) {
   BwdPlan p;
   const long rows = (long)d->Mq * (d->heads / d->kv_heads);
   p.nwq = rows >= 96L * d->B ? 4 : 1, p.nwk = d->Mk >= 96L * d->B ? 4 : 1;
   p.tiles_q = (int)(rows / (32 * p.nwq)) + d->B;
   p.tiles_k = d->Mk / (32 * p.nwk) + d->B;
   const long blocks = (long)p.tiles_k * d->kv_heads;
-  long n = blocks < 512 ? (768 + blocks - 1) / blocks : 1;
-  const long most = rows / d->B / 512;
+  long n = blocks < 512 ? (1024 + blocks - 1) / blocks : 1;
+  const long most = rows / d->B / (dt == OGV_BF16 ? 512 : 32);
   if (n > most) n = most;
   p.nsplit = (int)(n < 1 ? 1 : n > 16 ? 16 : n);
   return p;
@@ -353,7 +354,7 @@ using namespace ogv;
 
 extern "C" size_t ogv_packed_attn_bwd_ws_bytes(const ogv_packed_desc* d, ogv_dtype dt) {
   if (packed_check("ogv_packed_attn_bwd_ws_bytes", d, dt) != OGV_OK) return 0;
-  const BwdPlan p = bwd_plan(d);
+  const BwdPlan p = bwd_plan(d, dt);
   const size_t stat = ((size_t)d->Mq * d->heads * 2 + 3) & ~(size_t)3;
   return (stat + (p.nsplit > 1 ? (size_t)p.nsplit * 2 * d->Mk * d->kv_heads * d->D : 0)) * sizeof(float);
 }
@@ -370,7 +371,7 @@ extern "C" int ogv_packed_attn_bwd(const void* dout, const void* q, const void* 
   a.q = q, a.k = k, a.v = v, a.o = out, a.dout = dout, a.lse = const_cast<float*>(lse), a.rowstat = (float2*)ws;
   a.cu_q = cu_q, a.cu_k = cu_k, a.dq = dq, a.dk = dk, a.dv = dv;
   a.part_o = (float*)ws + (((size_t)d->Mq * d->heads * 2 + 3) & ~(size_t)3);
-  const BwdPlan p = bwd_plan(d);
+  const BwdPlan p = bwd_plan(d, dt);
   hipStream_t s = as_stream(stream);
 #define OGV_BWD(T)                                      \
   if (d->D <= 32) bwd_launch<T, 32>(p, a, s);           \

@@ -143,11 +143,14 @@ class _PackedAttention(torch.autograd.Function):
         ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
         ctx.meta = (causal, scale)
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _dlse):
+        if dout is None:
+            return (None,) * 7
         q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         _attn_bwd(_heads3(dout.to(q.dtype)), q, k, v, out, lse, cu_q, cu_k, *ctx.meta, dq, dk, dv)
@@ -374,6 +377,15 @@ def _norm_fwd(f, x, gate, rs, post_w, post_b, pre_w, pre_b, meta, stats=None):
     return y if h is None else (y, h)
 
 
+def _rows(g, like):
+    """A gradient as contiguous rows of the activations' type."""
+    if g is None:
+        return None
+    if g.dtype is not like.dtype:
+        g = g.to(like.dtype)
+    return g if g.is_contiguous() else g.contiguous()
+
+
 class _GatedNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, f, x, gate, rs, post_w, post_b, pre_w, pre_b, meta):
@@ -391,7 +403,7 @@ class _GatedNorm(torch.autograd.Function):
         if dy is None and dh is None:
             return (None,) * 9
         M, C = f.shape
-        dy, dh = (None if g is None else g.to(f.dtype).contiguous() for g in (dy, dh))
+        dy, dh = _rows(dy, f), _rows(dh, f)
         df, dx = torch.empty_like(f), torch.empty_like(f)
         sums = torch.empty((5, C), dtype=torch.float32, device=f.device)
         dgate = torch.empty_like(gate) if gate is not None and ctx.meta[2] > 1 else None
@@ -405,10 +417,11 @@ class _GatedNorm(torch.autograd.Function):
         else:
             sums.zero_()
             dgate = torch.zeros_like(gate) if dgate is not None else None
+        g, w1, b1, w0, b0 = sums.unbind(0)
         if gate is not None and dgate is None:
-            dgate = sums[0].view(gate.shape)
-        pick = lambda p, i: None if p is None else sums[i]  # noqa: E731
-        return (df, dx, dgate, None, pick(post_w, 3), pick(post_b, 4), pick(pre_w, 1), pick(pre_b, 2), None)
+            dgate = g if gate.ndim == 1 else g.view(gate.shape)
+        return (df, dx, dgate, None, None if post_w is None else w0, None if post_b is None else b0,
+                None if pre_w is None else w1, None if pre_b is None else b1, None)
 
 
 def gated_residual_norm(branch, residual, gate=None, row_scale=None, rps=1, alpha=1.0, post_norm=None, post_weight=None,

@@ -103,7 +103,7 @@ def test_attention_few_rows_many_keys(dtype, lq, lk, h, hkv):
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=str)
 @pytest.mark.parametrize("D", [32, 64, 96, 128])
-@pytest.mark.parametrize("h,hkv,lengths", [(3, 1, (900, 700)), (4, 1, (1100,)), (2, 2, (1400, 1700))], ids=str)
+@pytest.mark.parametrize("h,hkv,lengths", [(3, 1, (900, 700)), (4, 1, (1100,)), (2, 2, (1400, 1700)), (2, 1, (40, 70))], ids=str)
 def test_attention_rows_split_for_keys(dtype, D, h, hkv, lengths):
     """Few key tiles and many rows: the rows of dk and dv are split between workgroups and their sums joined."""
     import ctypes
@@ -111,7 +111,8 @@ def test_attention_rows_split_for_keys(dtype, D, h, hkv, lengths):
     import ogv._lib as L
     m = sum(lengths)
     d = L.PackedDesc(B=len(lengths), Mq=m, Mk=m, heads=h, kv_heads=hkv, D=D, scale=1.0)
-    assert L.load().ogv_packed_attn_bwd_ws_bytes(ctypes.byref(d), 1 if dtype == BF else 0) > 8 * m * h + 16
+    split = L.load().ogv_packed_attn_bwd_ws_bytes(ctypes.byref(d), 1 if dtype == BF else 0) > 8 * m * h + 16
+    assert split == (dtype == F32 or m > 1000)
     q, k, v, do = _qkv(m, m, h, hkv, D, dtype, D + h)
     for causal in (False, True):
         _check(q, k, v, lengths, lengths, causal, dout=do)
@@ -167,9 +168,11 @@ def test_attention_rows_behind_the_last_sequence(dtype, causal):
     qd, kd, vd = tail(q), tail(k), tail(v)
     out, lse = packed_attention(qd, kd, vd, cu, causal=causal, return_lse=True)
     got = torch.autograd.grad(out, (qd, kd, vd), tail(do).detach())
+    ref = R.attention(q, k, v, lengths, lengths, causal, 40**-0.5, dtype, do)   # (other sizes may take another split)
+    for a, n in zip((out, *got), ("out", "dq", "dk", "dv")):
+        _near(a[:103], *ref[n], n)
+        assert (a[103:] == 0).all()
     want = _check(q, k, v, lengths, lengths, causal, dout=do)
-    for a, b in zip((out, *got), want):
-        assert torch.equal(a[:103], b) and (a[103:] == 0).all()
     assert (lse[103:] == -math.inf).all()
     # NaN and infinities in the first sequence stay there
     for t in (q, k, v):
