@@ -149,10 +149,12 @@ template <typename P> __device__ __forceinline__ const char* uniform_ptr(const P
   return reinterpret_cast<const char*>(((uint64_t)hi << 32) | lo);
 }
 
+constexpr unsigned NO_CHUNK = ~0u;   // a chunk past the head: not copied, its place in the tile holds zeros (clear_tiles)
+
 // Copies ROWS rows of a strided tensor into an LDS tile, straight from global memory to LDS (no registers): one
 // instruction of a wave fills 64 consecutive chunks, so the swizzle is in the addresses that the lanes read.  Rows past
-// the last one repeat it and chunks past the head repeat the first: whoever uses the tile masks their products.
-// Offsets inside a tile are 32-bit (row strides are below 2^24 elements), the tile's base is a uniform pointer.
+// the last one repeat it: whoever uses the tile masks their products.  Offsets inside a tile are 32-bit (row strides are
+// below 2^24 elements), the tile's base is a uniform pointer.
 template <typename T, int D, int ROWS, int NW> struct TileCopy {
   using F = Frag<T, D>;
   static constexpr int NI = ROWS * F::NC / (64 * NW);
@@ -160,7 +162,7 @@ template <typename T, int D, int ROWS, int NW> struct TileCopy {
   unsigned off[NI];   // of this lane's chunks: row * stride + chunk, bytes
   static __device__ __forceinline__ unsigned place(int slot, int last, int Dlive, long stride) {
     const int row = slot / F::NC, ch = (slot - row * F::NC) ^ swz<F::RB>(row);
-    return (unsigned)min(row, last) * (unsigned)(stride * sizeof(T)) + (ch * F::E < Dlive ? ch * 16 : 0);
+    return ch * F::E < Dlive ? (unsigned)min(row, last) * (unsigned)(stride * sizeof(T)) + ch * 16 : NO_CHUNK;
   }
   __device__ __forceinline__ void init(int wave, int lane, int Dlive, long stride) {
 #pragma unroll
@@ -169,16 +171,24 @@ template <typename T, int D, int ROWS, int NW> struct TileCopy {
   // rows 0 .. ROWS - 1 behind base, of which `left` >= 1 exist
   __device__ __forceinline__ void load(const T* base, long stride, int left, char* tile, int wave, int lane, int Dlive) const {
     const char* b = uniform_ptr(base);
-    if (left >= ROWS) {
+    if (left >= ROWS && Dlive == D) {
 #pragma unroll
       for (int n = 0; n < NI; ++n) copy16(b, off[n], tile + (n * NW + wave) * 1024);
     } else {
 #pragma unroll
-      for (int n = 0; n < NI; ++n)
-        copy16(b, place((n * NW + wave) * 64 + lane, left - 1, Dlive, stride), tile + (n * NW + wave) * 1024);
+      for (int n = 0; n < NI; ++n) {
+        const unsigned at = left >= ROWS ? off[n] : place((n * NW + wave) * 64 + lane, left - 1, Dlive, stride);
+        if (at != NO_CHUNK) copy16(b, at, tile + (n * NW + wave) * 1024);
+      }
     }
   }
 };
+
+// Zeros for the chunks that no copy writes; once, before the first copy.
+template <int BYTES, int NT> __device__ __forceinline__ void clear_tiles(char* tiles, int tid) {
+  for (int i = tid; i < BYTES / 16; i += NT) reinterpret_cast<uint4*>(tiles)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+}
 
 // Keeps the compiler from running a wave-uniform branch's body always and selecting its results.
 __device__ __forceinline__ void rare_branch() { asm volatile(""); }

@@ -57,6 +57,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dq_ker
 
   int h, t;
   if (!head_tile(a.d, a.hkv, a.tiles, h, t)) return;
+  if (a.D < D) clear_tiles<4 * TB, NW * 64>(tiles, tid);
   const Seq sq = find_tile(a.cu_q, a.cu_k, a.B, a.Mq, a.Mk, a.G, BM, a.tiles - 1 - t, lane);
   const int k0 = sq.start2, lk = sq.len2;
   const int rows = sq.len * a.G, r0 = sq.tile * BM;
@@ -182,6 +183,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dkv_ke
 
   int h, t;
   if (!head_tile(a.d, a.hkv, a.tiles * a.nsplit, h, t)) return;
+  if (a.D < D) clear_tiles<4 * TB, NT>(tiles, tid);
+  if (VL && a.D < D) clear_tiles<sizeof(Vl), NT>(Vl, tid);
   const int split = t % a.nsplit;
   const Seq sk = find_tile(a.cu_k, a.cu_q, a.B, a.Mk, a.Mq, 1, BM, t / a.nsplit, lane);
   const int q0 = sk.start2, lq = sk.len2;
@@ -204,9 +207,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dkv_ke
   auto place = [&](int n, int rt, int p0, int last, unsigned& oq, unsigned& og) {
     const int slot = (n * NW + wave) * 64 + lane, row = slot / F::NC, ch = (slot - row * F::NC) ^ swz<RB>(row);
     const int rr = min(rt + row, last), pos = group_div(rr, a.G, a.gmagic);
-    const unsigned hg = (unsigned)(rr - pos * a.G), dp = (unsigned)(pos - p0), col = ch * E < a.D ? ch * 16 : 0;
+    const unsigned hg = (unsigned)(rr - pos * a.G), dp = (unsigned)(pos - p0), col = ch * 16;
     oq = dp * (unsigned)(a.rq * sizeof(T)) + hg * (unsigned)(a.hsq * sizeof(T)) + col;
     og = dp * (unsigned)(a.rdo * sizeof(T)) + hg * (unsigned)(a.hsdo * sizeof(T)) + col;
+    if (ch * E >= a.D) oq = NO_CHUNK;
   };
   unsigned oq[NI], og[NI];   // of a whole step whose first row is its query's first head (always, where G divides BN)
 #pragma unroll
@@ -223,8 +227,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dkv_ke
       if (BN * F::NC % NT != 0 && (n * NW + wave) * 64 >= BN * F::NC) break;   // (uniform in a wave)
       unsigned x = oq[n], y = og[n];
       if (!whole) place(n, rt, p0, rows - 1, x, y);
-      copy16(qt, x, tiles + at + (n * NW + wave) * 1024);
-      copy16(gt, y, tiles + at + TB + (n * NW + wave) * 1024);
+      if (a.D == D || x != NO_CHUNK) {
+        copy16(qt, x, tiles + at + (n * NW + wave) * 1024);
+        copy16(gt, y, tiles + at + TB + (n * NW + wave) * 1024);
+      }
     }
     if (tid < BN) {
       const int rr = min(rt + tid, rows - 1), pos = group_div(rr, a.G, a.gmagic);
@@ -241,13 +247,6 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dkv_ke
       TileCopy<T, D, BM, NW> vc;
       vc.init(wave, lane, a.D, a.rv);
       vc.load((const T*)a.v + (long)(sk.start + j0) * a.rv + (long)h * a.hsv, a.rv, sk.len - j0, Vl, wave, lane, a.D);
-      if (a.D < D) {   // dout's chunks past the head are not zero, so these have to be
-        tiles_ready();
-        for (int i = tid; i < BM * F::NC; i += NT) {
-          const int row = i / F::NC, ch = i - row * F::NC;
-          if (ch * E >= a.D) *reinterpret_cast<uint4*>(Vl + row * RB + ((ch ^ swz<RB>(row)) << 4)) = make_uint4(0, 0, 0, 0);
-        }
-      }
     }
     const T* kp = (const T*)a.k + (long)(sk.start + (live ? j : j0)) * a.rk + (long)h * a.hsk;
     const T* vp = (const T*)a.v + (long)(sk.start + (live ? j : j0)) * a.rv + (long)h * a.hsv;

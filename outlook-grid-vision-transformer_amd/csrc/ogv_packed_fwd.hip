@@ -194,6 +194,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_fwd_ke
   constexpr int TB = (sizeof(T) == 2 && NW > 1 ? 64 : 32) * Frag<T, D>::RB;
   __shared__ __attribute__((aligned(16))) char tiles[4 * TB];
   const int lane = threadIdx.x & 63;
+  if (a.D < D) clear_tiles<4 * TB, NW * 64>(tiles, threadIdx.x);
   if (SPLIT) {   // every piece of work, head by head
     for (int n = blockIdx.x;; n += gridDim.x) {
       Piece p;
@@ -297,6 +298,9 @@ int packed_check(const char* what, const ogv_packed_desc* d, ogv_dtype dt) {
               "%s: grid too large", what);
   const long al = 16 / (dt == OGV_BF16 ? 2 : 4);
   for (int i = 0; i < OGV_PACKED_TENSORS; ++i) {
+    // (offsets inside a tile of 64 rows, and between the heads of a group, are 32-bit)
+    OGV_REQUIRE(G == 1 || (i != 0 && i != 4) || d->head[i] < (1L << 28) / G, "%s: head stride %d = %lld is too large", what, i,
+                (long long)d->head[i]);
     OGV_REQUIRE(d->row[i] < (1 << 24), "%s: row stride %d = %lld is too large (below 2^24 elements)", what, i, (long long)d->row[i]);
     OGV_REQUIRE(d->row[i] >= 0 && d->head[i] >= 0 && d->row[i] % al == 0 && d->head[i] % al == 0,
                 "%s: stride %d (row %lld, head %lld) must be non-negative multiples of 16 bytes", what, i,

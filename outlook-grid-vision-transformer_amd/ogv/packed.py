@@ -72,11 +72,13 @@ def _ws(nbytes, like):
     return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
 
 
-def _heads3(t):
-    """A [rows, heads, D] tensor the kernels can address (unit last stride, 16-byte rows, heads and base), else a copy."""
+def _heads3(t, group=1):
+    """A [rows, heads, D] tensor the kernels can address (unit last stride, 16-byte rows, heads and base, strides inside a
+    tile and inside a group of query heads within 32 bits), else a copy."""
     al = 16 // t.element_size()
     (m, h, d), (sm, sh, sd) = t.shape, t.stride()
-    if m > 1 and sm % al or h > 1 and sh % al or d > 1 and sd != 1 or t.data_ptr() % 16:
+    if (m > 1 and (sm % al or sm >= 1 << 24) or h > 1 and (sh % al or group > 1 and sh >= (1 << 28) // group)
+            or d > 1 and sd != 1 or t.data_ptr() % 16):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -153,7 +155,7 @@ class _PackedAttention(torch.autograd.Function):
             return (None,) * 7
         q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        _attn_bwd(_heads3(dout.to(q.dtype)), q, k, v, out, lse, cu_q, cu_k, *ctx.meta, dq, dk, dv)
+        _attn_bwd(_heads3(dout.to(q.dtype), q.shape[1] // k.shape[1]), q, k, v, out, lse, cu_q, cu_k, *ctx.meta, dq, dk, dv)
         return dq, dk, dv, None, None, None, None
 
 
@@ -200,7 +202,7 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal=False, scale=None, return_
         raise ValueError(f"{what}: cu_q has {cu_q.numel()} offsets, cu_k {cu_k.numel()}")
     _device(what, q, k, v, cu_q, cu_k)
     fn = _PackedAttention.apply if _grad(q, k, v) else _attn_fwd
-    out, lse = fn(_heads3(q), _heads3(k), _heads3(v), cu_q, cu_k, bool(causal), scale)
+    out, lse = fn(_heads3(q, q.shape[1] // k.shape[1]), _heads3(k), _heads3(v), cu_q, cu_k, bool(causal), scale)
     return (out, lse) if return_lse else out
 
 

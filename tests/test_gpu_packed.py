@@ -205,6 +205,20 @@ def test_attention_masked_keys_of_any_size():
     assert (out.double().cpu() - mean).abs().max() <= 2.0**-24 * 64 * v.abs().max()
 
 
+@pytest.mark.parametrize("D", [24, 32, 72])
+@pytest.mark.parametrize("dtype", [BF, F32], ids=str)
+def test_attention_key_of_minus_infinity(dtype, D):
+    """A key whose score is -inf for every query weighs nothing, with every head size (padded or not)."""
+    from ogv.packed import packed_attention
+    q, k, v, _ = _qkv(50, 50, 2, 1, D, dtype, D)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    keep = torch.arange(50) != 5
+    ref = R.attention(q, k[keep], v[keep], (50,), (49,), False, D**-0.5, dtype)
+    k[5, :, 0] = -math.inf
+    out = packed_attention(q.to(DEV), k.to(DEV), v.to(DEV), R.offsets((50,)).to(DEV))
+    _near(out, *ref["out"])
+
+
 def test_attention_bad_offsets_stay_inside():
     """Offsets past the rows are clamped, a decreasing pair is an empty sequence: no row outside is read or written."""
     from ogv.packed import packed_attention

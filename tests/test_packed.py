@@ -148,6 +148,10 @@ def test_c_abi_refuses_before_any_launch():
     d = L.PackedDesc(B=2, Mq=10, Mk=10, heads=4, kv_heads=2, D=16, scale=0.25)
     d.row[1] = 12
     assert "multiples of 16" in fwd(ctypes.byref(d))[1]
+    d.row[1] = 1 << 24
+    assert "too large" in fwd(ctypes.byref(d))[1]
+    d.row[1], d.head[0] = 32, 1 << 28      # two query heads share a key head: their distance is a 32-bit offset
+    assert "too large" in fwd(ctypes.byref(d))[1]
 
     def rot(**more):
         d = L.RotaryDesc(M=4, D=16, axes=2, theta=1e4)
