@@ -40,18 +40,22 @@ def _dtype(what, first, *ts):
 
 
 def _device(what, first, *ts):
-    dev = first.device
+    dev = first.get_device()   # (-1: not on a device)
     for t in (first, *ts):
         if t is not None:
-            if not t.is_cuda:
+            if t.get_device() < 0:
                 raise RuntimeError(f"{what}: the MI355X kernels need HIP device tensors (got {t.device}); "
                                    f"this framework has no CPU execution path")
-            if t.device != dev:
-                raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+            if t.get_device() != dev:
+                raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
 
 
 def _grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _ptr(t):
@@ -60,7 +64,7 @@ def _ptr(t):
 
 def _launch(fn, name, like, *args):
     """Call the C-ABI on the current stream of `like`'s device, with that device current."""
-    dev = like.device.index
+    dev = like.get_device()
     if dev == torch.cuda.current_device():
         check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)), name)
     else:
@@ -255,21 +259,29 @@ class _AxialRotary(torch.autograd.Function):
         return (None, None, *outs)
 
 
-def _check_rotary(what, D, positions, sections, theta, interleaved, rows):
+@functools.lru_cache(1024)
+def _rotary_meta(what, D, sections, theta, interleaved):
     sections = tuple(int(n) for n in sections)
     if not (1 <= len(sections) <= 4 and all(n > 0 for n in sections)):
         raise ValueError(f"{what}: sections must be 1 to 4 positive pair counts, got {sections}")
     if not (D % 2 == 0 and D <= 128 and 2 * sum(sections) <= D):
         raise ValueError(f"{what}: {sum(sections)} pairs need an even head_dim of at "
                          f"least {2 * sum(sections)} (and at most 128), got {D}")
-    if not (positions.dtype in (torch.int32, torch.float32)):
-        raise TypeError(f"{what}: positions must be int32 or float32, got {positions.dtype}")
-    if not (positions.shape == (rows, len(sections))):
-        raise ValueError(f"{what}: positions [rows, axes] = [{rows}, {len(sections)}] expected, got {tuple(positions.shape)}")
     theta = float(theta)
-    if not (0.0 < theta < math.inf):
+    if not 0.0 < theta < math.inf:
         raise ValueError(f"{what}: theta must be positive and finite, got {theta}")
-    return positions.detach() if positions.is_contiguous() else positions.detach().contiguous(), (sections, theta, bool(interleaved))
+    return sections, theta, bool(interleaved)
+
+
+def _check_rotary(what, D, positions, sections, theta, interleaved, rows):
+    meta = _rotary_meta(what, D, tuple(sections), theta, interleaved)
+    if positions.dtype is not torch.int32 and positions.dtype is not torch.float32:
+        raise TypeError(f"{what}: positions must be int32 or float32, got {positions.dtype}")
+    if positions.shape != (rows, len(meta[0])):
+        raise ValueError(f"{what}: positions [rows, axes] = [{rows}, {len(meta[0])}] expected, got {tuple(positions.shape)}")
+    if positions.requires_grad:
+        positions = positions.detach()
+    return positions if positions.is_contiguous() else positions.contiguous(), meta
 
 
 def axial_rotary(q, k, positions, sections, theta=10000.0, interleaved=False):
