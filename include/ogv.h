@@ -209,7 +209,8 @@ int ogv_layernorm_bwd(const void* dy, const void* x, const float* gamma, const f
  *   not decreasing; the first offset is taken as 0, all are clamped to [0, M]).  Any length may be 0.
  *   causal: key j of a sequence is seen by its query i where j <= i + keys - queries.
  *   A row that sees no key, and a row behind the last sequence: out 0, lse -inf, gradients 0.
- * Backward: dout, dq like q; dk, dv like k; out and lse as the forward wrote them.
+ * out_lo, like out (NULL: not wanted; bf16 only): what the rounding took from out, for a backward.
+ * Backward: dout, dq like q; dk, dv like k; out, out_lo (NULL: taken as 0) and lse as the forward wrote them.
  * ws >= the *_ws_bytes query (forward: 0 bytes, may be NULL, unless the keys are split).  Deterministic.
  * The backward forms the weights again from lse in fp32: a weight's relative error is about 2^-23 |scale q . k|.
  * A non-finite value in v reaches its own sequence only.  bf16 or fp32, D % 8 == 0, D <= 128, scale > 0.
@@ -222,10 +223,10 @@ typedef struct {
 } ogv_packed_desc;
 size_t ogv_packed_attn_fwd_ws_bytes(const ogv_packed_desc* d, ogv_dtype dt);
 int ogv_packed_attn_fwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* out,
-                        float* lse, void* ws, const ogv_packed_desc* d, ogv_dtype dt, void* stream);
+                        void* out_lo, float* lse, void* ws, const ogv_packed_desc* d, ogv_dtype dt, void* stream);
 size_t ogv_packed_attn_bwd_ws_bytes(const ogv_packed_desc* d, ogv_dtype dt);
 int ogv_packed_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
-                        const float* lse, const int* cu_q, const int* cu_k, void* dq, void* dk, void* dv, void* ws,
+                        const void* out_lo, const float* lse, const int* cu_q, const int* cu_k, void* dq, void* dk, void* dv, void* ws,
                         const ogv_packed_desc* d, ogv_dtype dt, void* stream);
 
 /* ---------------------------------------------------------------------------------------------

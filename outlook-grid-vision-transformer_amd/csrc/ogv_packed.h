@@ -52,8 +52,8 @@ __device__ __forceinline__ bool head_tile(const Deal d, int hkv, int tiles, int&
 }
 
 struct PackedArgs {
-  const void *q, *k, *v, *o, *dout;   // o: forward's output (read by the backward)
-  void *out, *dq, *dk, *dv;
+  const void *q, *k, *v, *o, *o_lo, *dout;   // o, o_lo: forward's outputs (read by the backward)
+  void *out, *out_lo, *dq, *dk, *dv;
   float* lse;
   float2* rowstat;                    // backward: lse * log2(e) (+inf where no key is seen) and delta of a row
   const int *cu_q, *cu_k;

@@ -7,7 +7,9 @@
 // Two kernels, each owning the rows it writes, so no sum depends on the order of workgroups: dq walks the
 // keys of a row block (and forms delta), dk / dv walk the rows -- of all query heads that share the key head --
 // of a key block.  That computes the scores and dp twice (7 products for 5) and needs no atomics and no zeroed
-// accumulators.  P and dS are rounded to bf16 for their products; scores, dp, delta and sums are fp32.
+// accumulators.  P and dS are rounded to bf16 for their products; scores, dp, delta and sums are fp32.  delta is taken
+// from o and what its rounding left (out_lo): from the rounded o alone its error, common to a row's keys, was larger
+// than dS's rounding (dq of short sequences: 0.0032 off in 2-norm instead of 0.0024).
 #include "ogv_packed.h"
 
 #include <initializer_list>
@@ -97,11 +99,12 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dq_ker
       if (live && d < a.D) {
         qf[kk].u = *reinterpret_cast<const uint4*>(qp + d);
         gf[kk].u = *reinterpret_cast<const uint4*>(gp + d);
-        Chunk oc;
+        Chunk oc, lc = zero_chunk();
         oc.u = *reinterpret_cast<const uint4*>(op + d);
         if constexpr (sizeof(T) == 2) {
+          if (a.o_lo) lc.u = *reinterpret_cast<const uint4*>((const T*)a.o_lo + row * a.ro + head * a.hso + d);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[kk].h[e], (float)oc.h[e], delta);
+          for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[kk].h[e], (float)oc.h[e] + (float)lc.h[e], delta);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e) delta = fmaf(gf[kk].f[e], oc.f[e], delta);
@@ -358,16 +361,16 @@ extern "C" size_t ogv_packed_attn_bwd_ws_bytes(const ogv_packed_desc* d, ogv_dty
   return (stat + (p.nsplit > 1 ? (size_t)p.nsplit * 2 * d->Mk * d->kv_heads * d->D : 0)) * sizeof(float);
 }
 
-extern "C" int ogv_packed_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
+extern "C" int ogv_packed_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const void* out_lo,
                                    const float* lse, const int* cu_q, const int* cu_k, void* dq, void* dk, void* dv,
                                    void* ws, const ogv_packed_desc* d, ogv_dtype dt, void* stream) {
   if (int rc = packed_check("ogv_packed_attn_bwd", d, dt)) return rc;
   OGV_REQUIRE(dout && q && out && lse && cu_q && cu_k && dq && ws && (d->Mk == 0 || (k && v && dk && dv)),
               "ogv_packed_attn_bwd: null pointer");
-  OGV_REQUIRE(aligned16({dout, q, k, v, out, dq, dk, dv, ws}), "ogv_packed_attn_bwd: pointers must be 16-byte aligned");
+  OGV_REQUIRE(aligned16({dout, q, k, v, out, out_lo, dq, dk, dv, ws}), "ogv_packed_attn_bwd: pointers must be 16-byte aligned");
   PackedArgs a;
   packed_args(d, a);
-  a.q = q, a.k = k, a.v = v, a.o = out, a.dout = dout, a.lse = const_cast<float*>(lse), a.rowstat = (float2*)ws;
+  a.q = q, a.k = k, a.v = v, a.o = out, a.o_lo = out_lo, a.dout = dout, a.lse = const_cast<float*>(lse), a.rowstat = (float2*)ws;
   a.cu_q = cu_q, a.cu_k = cu_k, a.dq = dq, a.dk = dk, a.dv = dv;
   a.part_o = (float*)ws + (((size_t)d->Mq * d->heads * 2 + 3) & ~(size_t)3);
   const BwdPlan p = bwd_plan(d, dt);

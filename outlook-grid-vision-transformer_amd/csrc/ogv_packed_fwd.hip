@@ -8,7 +8,8 @@
 // transposed (S^T = K Q^T), so a row's scores lie in two lanes and its maximum, sum and rescaling are
 // lane-local but for one exchange, and P^T feeds O^T += V^T P^T from registers.  K and V tiles pass
 // through LDS once per workgroup.  Scores, maximum, sum and O are fp32; P is rounded to bf16 for the second
-// product (relative error 2^-9 per weight, independent from key to key, below the output's own rounding).
+// product (a relative error of at most 2^-8 per weight, independent from key to key; the output's own rounding is as
+// large).  For a backward, what rounding took from o is kept too (out_lo): see delta there.
 #include "ogv_packed.h"
 
 #include <initializer_list>
@@ -186,6 +187,16 @@ __device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* tiles, int h
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);   // (NaN stays NaN)
   store_cols<T, D>((T*)a.out + (long)(start + pos) * a.ro + (long)(h * a.G + hg) * a.hso, o, inv, a.D, hf, out);
+  if (sizeof(T) == 2 && a.out_lo) {
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float x = o[db][i] * inv;
+        o[db][i] = x - (float)(T)x;
+      }
+    store_cols<T, D>((T*)a.out_lo + (long)(start + pos) * a.ro + (long)(h * a.G + hg) * a.hso, o, 1.f, a.D, hf, out);
+  }
   if (out && hf == 0) a.lse[orow] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
 }
 
@@ -241,6 +252,10 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const PackedArgs a) {
   const long q = row / a.hq;
   const float v[2] = {x, y};
   if (d < a.D) store_vec<T, 2>((T*)a.out + q * a.ro + (row - q * a.hq) * a.hso + d, v);
+  if (sizeof(T) == 2 && a.out_lo) {
+    const float lo[2] = {x - (float)(T)x, y - (float)(T)y};
+    if (d < a.D) store_vec<T, 2>((T*)a.out_lo + q * a.ro + (row - q * a.hq) * a.hso + d, lo);
+  }
   if (lane == 0) a.lse[row] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
 }
 
@@ -336,16 +351,16 @@ extern "C" size_t ogv_packed_attn_fwd_ws_bytes(const ogv_packed_desc* d, ogv_dty
 }
 
 extern "C" int ogv_packed_attn_fwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k,
-                                   void* out, float* lse, void* ws, const ogv_packed_desc* d, ogv_dtype dt,
+                                   void* out, void* out_lo, float* lse, void* ws, const ogv_packed_desc* d, ogv_dtype dt,
                                    void* stream) {
   if (int rc = packed_check("ogv_packed_attn_fwd", d, dt)) return rc;
   OGV_REQUIRE(q && cu_q && cu_k && out && lse && (d->Mk == 0 || (k && v)), "ogv_packed_attn_fwd: null pointer");
   const FwdPlan p = fwd_plan(d);
   OGV_REQUIRE(p.nsplit == 1 || ws, "ogv_packed_attn_fwd: null workspace");
-  OGV_REQUIRE(aligned16({q, k, v, out, ws}), "ogv_packed_attn_fwd: pointers must be 16-byte aligned");
+  OGV_REQUIRE(aligned16({q, k, v, out, out_lo, ws}), "ogv_packed_attn_fwd: pointers must be 16-byte aligned");
   PackedArgs a;
   packed_args(d, a);
-  a.q = q, a.k = k, a.v = v, a.cu_q = cu_q, a.cu_k = cu_k, a.out = out, a.lse = lse;
+  a.q = q, a.k = k, a.v = v, a.cu_q = cu_q, a.cu_k = cu_k, a.out = out, a.out_lo = out_lo, a.lse = lse;
   a.d = deal(d->kv_heads, p.tiles), a.tiles = p.tiles, a.nsplit = p.nsplit, a.chunk = p.chunk;
   const size_t n = (size_t)p.nsplit * d->Mq * d->heads;
   a.part_o = (float*)ws;

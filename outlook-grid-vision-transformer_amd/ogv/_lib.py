@@ -110,9 +110,9 @@ SIGNATURES = {
     "ogv_grid_attn_fwd": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _f, _i, _p]),
     "ogv_grid_attn_bwd": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _f, _i, _p]),
     "ogv_packed_attn_fwd_ws_bytes": (_sz, [_PKD, _i]),
-    "ogv_packed_attn_fwd": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _PKD, _i, _p]),
+    "ogv_packed_attn_fwd": (_i, [_p] * 9 + [_PKD, _i, _p]),
     "ogv_packed_attn_bwd_ws_bytes": (_sz, [_PKD, _i]),
-    "ogv_packed_attn_bwd": (_i, [_p] * 12 + [_PKD, _i, _p]),
+    "ogv_packed_attn_bwd": (_i, [_p] * 13 + [_PKD, _i, _p]),
     "ogv_axial_rotary": (_i, [_p, _p, _p, _p, _p, _PRD, _i, _p]),
     "ogv_gated_norm_fwd": (_i, [_p] * 11 + [_PND, _i, _p]),
     "ogv_gated_norm_bwd_ws_bytes": (_sz, [_PND, _i]),

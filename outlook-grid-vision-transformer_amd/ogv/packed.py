@@ -108,7 +108,8 @@ def _packed_desc(B, Mq, Mk, heads, kv_heads, D, causal, scale, dt, *strides):
     return r, lib.ogv_packed_attn_fwd_ws_bytes(r, dt), lib.ogv_packed_attn_bwd_ws_bytes(r, dt)
 
 
-def _attn_fwd(q, k, v, cu_q, cu_k, causal, scale):
+def _attn_fwd(q, k, v, cu_q, cu_k, causal, scale, lo=None):
+    """out and lse; lo (like out) gets what the rounding took from out."""
     dt = _dtype("ogv.packed_attention", q, k, v)
     Mq, heads, D = q.shape
     out = torch.empty((Mq, heads, D), dtype=q.dtype, device=q.device)
@@ -117,16 +118,22 @@ def _attn_fwd(q, k, v, cu_q, cu_k, causal, scale):
         return out, lse
     B = cu_q.shape[0] - 1
     if B == 0:   # no sequence at all: every row is behind the last one
+        if lo is not None:
+            lo.zero_()
         return out.zero_(), lse.fill_(-math.inf)
     d, ws, _ = _packed_desc(B, Mq, k.shape[0], heads, k.shape[1], D, causal, scale, dt, _strides(q), _strides(k), _strides(v),
                             (heads * D, D))
     ws = _ws(ws, q)
     _launch(_lib.load().ogv_packed_attn_fwd, "ogv_packed_attn_fwd", q, _ptr(q), _ptr(k), _ptr(v), _ptr(cu_q), _ptr(cu_k),
-            _ptr(out), _ptr(lse), _ptr(ws), d, dt)
+            _ptr(out), _ptr(lo), _ptr(lse), _ptr(ws), d, dt)
     return out, lse
 
 
-def _attn_bwd(dout, q, k, v, out, lse, cu_q, cu_k, causal, scale, dq, dk, dv):
+def _lo(q):
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device) if q.dtype is torch.bfloat16 else None
+
+
+def _attn_bwd(dout, q, k, v, out, lo, lse, cu_q, cu_k, causal, scale, dq, dk, dv):
     """Writes dq, dk, dv (which may be strided)."""
     dt = _dtype("ogv.packed_attention", q, k, v, dout)
     Mq, heads, D = q.shape
@@ -139,14 +146,15 @@ def _attn_bwd(dout, q, k, v, out, lse, cu_q, cu_k, causal, scale, dq, dk, dv):
                             *(_strides(t) for t in (q, k, v, out, dout, dq, dk, dv)))
     ws = _ws(ws, q)
     _launch(_lib.load().ogv_packed_attn_bwd, "ogv_packed_attn_bwd", q, _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
-            _ptr(lse), _ptr(cu_q), _ptr(cu_k), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), d, dt)
+            _ptr(lo), _ptr(lse), _ptr(cu_q), _ptr(cu_k), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), d, dt)
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, causal, scale):
-        out, lse = _attn_fwd(q, k, v, cu_q, cu_k, causal, scale)
-        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
+        lo = _lo(q)
+        out, lse = _attn_fwd(q, k, v, cu_q, cu_k, causal, scale, lo)
+        ctx.save_for_backward(q, k, v, out, lo, lse, cu_q, cu_k)
         ctx.meta = (causal, scale)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -157,9 +165,9 @@ class _PackedAttention(torch.autograd.Function):
     def backward(ctx, dout, _dlse):
         if dout is None:
             return (None,) * 7
-        q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
+        q, k, v, out, lo, lse, cu_q, cu_k = ctx.saved_tensors
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        _attn_bwd(_heads3(dout.to(q.dtype), q.shape[1] // k.shape[1]), q, k, v, out, lse, cu_q, cu_k, *ctx.meta, dq, dk, dv)
+        _attn_bwd(_heads3(dout.to(q.dtype), q.shape[1] // k.shape[1]), q, k, v, out, lo, lse, cu_q, cu_k, *ctx.meta, dq, dk, dv)
         return dq, dk, dv, None, None, None, None
 
 
@@ -323,21 +331,22 @@ class _RotaryAttentionRows(torch.autograd.Function):
             turned = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
             _rotate((q, k), turned, positions, rot, False)
             q, k = turned
-        out, lse = _attn_fwd(q, k, v, cu, cu, causal, scale)
-        ctx.save_for_backward(qkv, *((q, k) if rot is not None else (None, None)), out, lse, cu, positions)
+        lo = _lo(q) if ctx.needs_input_grad[0] else None
+        out, lse = _attn_fwd(q, k, v, cu, cu, causal, scale, lo)
+        ctx.save_for_backward(qkv, *((q, k) if rot is not None else (None, None)), out, lo, lse, cu, positions)
         ctx.meta = (rot, heads, kv_heads, causal, scale)
         return out.flatten(1)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        qkv, q, k, out, lse, cu, positions = ctx.saved_tensors
+        qkv, q, k, out, lo, lse, cu, positions = ctx.saved_tensors
         rot, heads, kv_heads, causal, scale = ctx.meta
         q0, k0, v = _RotaryAttentionRows._split(qkv, heads, kv_heads)
         q, k = (q0, k0) if rot is None else (q, k)
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         dq, dk, dv = _RotaryAttentionRows._split(dqkv, heads, kv_heads)
-        _attn_bwd(_heads3(dout.to(qkv.dtype).unflatten(1, (heads, -1))), q, k, v, out, lse, cu, cu, causal, scale, dq, dk, dv)
+        _attn_bwd(_heads3(dout.to(qkv.dtype).unflatten(1, (heads, -1))), q, k, v, out, lo, lse, cu, cu, causal, scale, dq, dk, dv)
         if rot is not None:
             _rotate((dq, dk), (dq, dk), positions, rot, True)
         return dqkv, None, None, None, None, None, None, None

@@ -131,7 +131,7 @@ def test_c_abi_refuses_before_any_launch():
     def fwd(d, **p):
         a = dict(q=x, k=x, v=x, cu_q=x, cu_k=x, out=x, lse=x, ws=x, dt=1)
         a.update(p)
-        rc = lib.ogv_packed_attn_fwd(a["q"], a["k"], a["v"], a["cu_q"], a["cu_k"], a["out"], a["lse"], a["ws"], d, a["dt"], None)
+        rc = lib.ogv_packed_attn_fwd(a["q"], a["k"], a["v"], a["cu_q"], a["cu_k"], a["out"], None, a["lse"], a["ws"], d, a["dt"], None)
         return rc, lib.ogv_last_error().decode()
 
     for more, match in ((dict(B=0), "bad shape"), (dict(Mq=0), "bad shape"), (dict(Mk=-1), "bad shape"), (dict(heads=3), "multiple"),
@@ -140,11 +140,11 @@ def test_c_abi_refuses_before_any_launch():
         rc, msg = fwd(desc(**more))
         assert rc == L.OGV_ERR_ARG and match in msg, (more, rc, msg)
         assert lib.ogv_packed_attn_fwd_ws_bytes(desc(**more), 1) == 0 and lib.ogv_packed_attn_bwd_ws_bytes(desc(**more), 1) == 0
-        assert lib.ogv_packed_attn_bwd(x, x, x, x, x, x, x, x, x, x, x, x, desc(**more), 1, None) == L.OGV_ERR_ARG
+        assert lib.ogv_packed_attn_bwd(x, x, x, x, x, x, x, x, x, x, x, x, x, desc(**more), 1, None) == L.OGV_ERR_ARG
     assert fwd(desc(), dt=2)[0] == L.OGV_ERR_ARG
     assert "null" in fwd(desc(), lse=None)[1]
     assert "aligned" in fwd(desc(), k=odd)[1]
-    assert lib.ogv_packed_attn_fwd(x, x, x, x, x, x, x, x, None, 1, None) == L.OGV_ERR_ARG
+    assert lib.ogv_packed_attn_fwd(x, x, x, x, x, x, x, x, x, None, 1, None) == L.OGV_ERR_ARG
     d = L.PackedDesc(B=2, Mq=10, Mk=10, heads=4, kv_heads=2, D=16, scale=0.25)
     d.row[1] = 12
     assert "multiples of 16" in fwd(ctypes.byref(d))[1]
