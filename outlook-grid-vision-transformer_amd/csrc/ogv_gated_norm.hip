@@ -9,7 +9,10 @@
 //   dgate = sum s_b n dY   (dw, db) of a norm = sums of (g vhat, g) over the rows
 //   N'(g) = rstd (g w - [mean(g w)] - vhat mean(g w vhat))        ([.]: layer only)
 //
-// Bound by memory: forward f, x -> y, h (4 rows of C), backward f, x, dy, dh -> df, dx (6).  A row belongs to
+// Bound by memory: forward f, x -> y, h (4 rows of C), backward f, x, dy, dh -> df, dx (6): 65536 rows of 768, bf16, layer
+// norms on both sides take 90 us and 133 us, 4.5 TB/s (a large copy: 4.9); 12800 rows of 331, fp32, 15 and 26 us.  The
+// backward loads the next row while it works on one (with it and two sums for three gradients: 355 -> 133 us, as the
+// registers then leave two waves to a SIMD).  A row belongs to
 // G lanes (a part of a wave, a wave, or a workgroup) that keep it in registers through every reduction.
 // Column sums: each lane adds its columns over the workgroup's rows, one partial row per workgroup, then they are added
 // in a fixed order: no atomics.

@@ -10,6 +10,22 @@
 // through LDS once per workgroup.  Scores, maximum, sum and O are fp32; P is rounded to bf16 for the second
 // product (a relative error of at most 2^-8 per weight, independent from key to key; the output's own rounding is as
 // large).  For a backward, what rounding took from o is kept too (out_lo): see delta there.
+//
+// Split: four waves of 32 rows share the tiles (64 keys; 32 in fp32 and for one-wave workgroups of short sequences), two
+// workgroups to a CU for D = 128, three for D = 64.  A row tile's keys are walked in one piece where the row tiles fill
+// the chip; otherwise (single queries) they are cut into equal pieces whose partial results a second kernel joins.
+//
+// What bounds it, measured on one MI355X (a large bf16 matrix product reaches 1365 TFLOP/s):
+//   D = 128, causal, 16 heads on 4, sequences of 8191 and 5608: 405 us, 996 TFLOP/s.  Left out in turn, the first product
+//     saves 116 us, the second 133, the copies to LDS 61, the exponentials 7: the matrix instructions and the LDS reads that
+//     feed them (1 KB a product of 32 cycles, half the LDS rate from two waves a SIMD) do not overlap further.
+//   D = 64, 48 images of 196 to 1024 tokens, 12 heads: 91 us, 540 TFLOP/s.  29 us of it are the workgroups' ends (q read, out
+//     written: 78 MB), the rest is spread over the 16-cycle exponentials (42 us for all of them with the other vector
+//     instructions) and the latencies of 3 to 16 tiles a workgroup.
+//   One query for each of 64 sequences (up to 8192 keys), 16 heads on 2: 31 us for 100 MB of keys and values, 3.2 TB/s, of
+//     which the joining launch takes 5.
+// The next tile's scores are computed before this tile's exponentials (466 -> 431 us at D = 128), copies bypass the
+// registers (1318 -> 558), the reference of the weights moves lazily, heads are dealt evenly to the XCDs (558 -> 479).
 #include "ogv_packed.h"
 
 #include <initializer_list>

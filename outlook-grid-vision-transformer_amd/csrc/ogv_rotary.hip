@@ -5,7 +5,8 @@
 //   y1 = x1 cos - x2 sin,  y2 = x2 cos + x1 sin
 // The backward is the turn by the negative angle.  Dims from 2 * P on pass unchanged.
 //
-// Bound by memory: 2 * elements * size bytes, every element read and written once.  A workgroup forms the
+// Bound by memory: 2 * elements * size bytes, every element read and written once: 65536 tokens, 16 + 4 heads of 128, bf16
+// take 148 us a direction, 4.5 TB/s (a large copy: 4.9).  A workgroup forms the
 // sines and cosines of its tokens once in LDS and uses them for all heads of q and k.  Angles are kept in
 // turns and reduced to (-1/2, 1/2] in fp64 (a position of 10^5 leaves an fp32 angle with 2 decimal digits).
 #include "ogv_common.h"
