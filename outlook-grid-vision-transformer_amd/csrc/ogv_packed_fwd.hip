@@ -22,7 +22,7 @@
 //   D = 64, 48 images of 196 to 1024 tokens, 12 heads: 91 us, 540 TFLOP/s.  29 us of it are the workgroups' ends (q read, out
 //     written: 78 MB), the rest is spread over the 16-cycle exponentials (42 us for all of them with the other vector
 //     instructions) and the latencies of 3 to 16 tiles a workgroup.
-//   One query for each of 64 sequences (up to 8192 keys), 16 heads on 2: 31 us for 100 MB of keys and values, 3.2 TB/s, of
+//   One query for each of 64 sequences (up to 8192 keys), 16 heads on 2: 30.8 us for 100 MB of keys and values, 3.2 TB/s, of
 //     which the joining launch takes 5.
 // The next tile's scores are computed before this tile's exponentials (466 -> 431 us at D = 128), copies bypass the
 // registers (1318 -> 558), the reference of the weights moves lazily, heads are dealt evenly to the XCDs (558 -> 479).
@@ -282,14 +282,14 @@ struct FwdPlan {
 
 // Sequences that fill four waves' rows on average get them, others one wave per workgroup.  While the row tiles
 // would not fill the 256 CUs twice, the keys are split into pieces of equal size (not equal number: sequences
-// differ), about 1024 in all.
+// differ), about 800 in all (64 single queries, 97 thousand keys, 16 heads on 2 of 128: 30.8 us; 1024 31.5, 1500 32.9).
 static FwdPlan fwd_plan(const ogv_packed_desc* d) {
   FwdPlan p;
   const long rows = (long)d->Mq * (d->heads / d->kv_heads);
   p.nw = rows >= 96L * d->B ? 4 : 1;
   p.tiles = (int)(rows / (32 * p.nw)) + d->B;
   const long blocks = (long)p.tiles * d->kv_heads;
-  long chunk = ((long)d->Mk * blocks / d->B / 1024 + 63) & ~63L;   // keys read by all row tiles over 1024
+  long chunk = ((long)d->Mk * blocks / d->B / 800 + 63) & ~63L;   // keys read by all row tiles over 800
   if (chunk < 128) chunk = 128;
   p.chunk = (int)(chunk < (1 << 30) ? chunk : 1 << 30);
   const bool split = blocks < 512 && d->Mk / d->B >= 2 * chunk;

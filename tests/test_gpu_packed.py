@@ -88,7 +88,7 @@ def test_attention_other_queries_than_keys(dtype, lq, lk, causal):
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=str)
 @pytest.mark.parametrize("lq,lk,h,hkv", [((1,), (2500,), 2, 1), ((1, 1, 1, 1), (4000, 3, 900, 1), 8, 1), ((3,), (1999,), 3, 3),
-                                         ((40, 1), (1500, 1500), 2, 2)], ids=str)
+                                         ((40, 1), (1500, 1500), 2, 2), ((130,), (3000,), 1, 1), ((200, 3), (2100, 900), 2, 1)], ids=str)
 def test_attention_few_rows_many_keys(dtype, lq, lk, h, hkv):
     """The key axis is split between workgroups and joined."""
     import ctypes
@@ -99,6 +99,27 @@ def test_attention_few_rows_many_keys(dtype, lq, lk, h, hkv):
     assert L.load().ogv_packed_attn_fwd_ws_bytes(ctypes.byref(d), 1 if dtype == BF else 0) > 0
     for causal in (False, True):
         _check(q, k, v, lq, lk, causal, dout=do)
+
+
+@pytest.mark.parametrize("D", [40, 128])
+def test_attention_many_single_queries(D):
+    """More sequences than a wave has lanes, keys of every length among them 0 and 1, rows behind the last sequence."""
+    from ogv.packed import packed_attention
+    g = _gen(D)
+    lk = [0, 1, 2000] + [int(n) for n in torch.randint(1, 1300, (117,), generator=g)]
+    q, k, v, _ = _qkv(130, sum(lk), 2, 1, D, BF, 3)
+    out, lse = packed_attention(q.to(DEV), k.to(DEV), v.to(DEV), R.offsets([1] * 120).to(DEV), R.offsets(lk).to(DEV), return_lse=True)
+    ref = R.attention(q, k, v, [1] * 120, lk, False, D**-0.5, BF)
+    _near(out, *ref["out"])
+    _near(lse, *ref["lse"])
+    assert (out[120:] == 0).all()
+
+
+def test_attention_thousands_of_sequences():
+    lengths = [int(n) for n in torch.randint(0, 4, (5000,), generator=_gen(0))]
+    m = sum(lengths)
+    q, k, v, do = _qkv(m, m, 2, 1, 16, BF, 7)
+    _check(q, k, v, lengths, lengths, True, dout=do)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=str)
