@@ -76,22 +76,28 @@ def _ws(nbytes, like):
     return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
 
 
+def _addressable(shape, stride, al, group=1):
+    """Whether the kernels can address [rows, heads, D] of these strides: unit last stride, rows and heads at multiples of
+    al elements (16 bytes), offsets inside a tile and inside a group of query heads within 32 bits."""
+    (m, h, d), (sm, sh, sd) = shape, stride
+    return not (m > 1 and (sm % al or sm >= 1 << 24) or h > 1 and (sh % al or group > 1 and sh >= (1 << 28) // group)
+                or d > 1 and sd != 1)
+
+
 def _heads3(t, group=1):
-    """A [rows, heads, D] tensor the kernels can address (unit last stride, 16-byte rows, heads and base, strides inside a
-    tile and inside a group of query heads within 32 bits), else a copy."""
-    al = 16 // t.element_size()
-    (m, h, d), (sm, sh, sd) = t.shape, t.stride()
-    if (m > 1 and (sm % al or sm >= 1 << 24) or h > 1 and (sh % al or group > 1 and sh >= (1 << 28) // group)
-            or d > 1 and sd != 1 or t.data_ptr() % 16):
+    """t, or a contiguous copy where the kernels cannot address it."""
+    if t.data_ptr() % 16 or not _addressable(t.shape, t.stride(), 16 // t.element_size(), group):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _strides(t):
+def _row_head(shape, stride):
     """(row, head) strides; those of a size-1 dim are never used and may be anything in torch."""
-    m, h, _ = t.shape
-    sm, sh, _ = t.stride()
-    return (sm if m > 1 else 0, sh if h > 1 else 0)
+    return (stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0)
+
+
+def _strides(t):
+    return _row_head(t.shape, t.stride())
 
 
 # ------------------------------------------------------------------------------------------------
@@ -108,12 +114,12 @@ def _packed_desc(B, Mq, Mk, heads, kv_heads, D, causal, scale, dt, *strides):
     return r, lib.ogv_packed_attn_fwd_ws_bytes(r, dt), lib.ogv_packed_attn_bwd_ws_bytes(r, dt)
 
 
-def _attn_fwd(q, k, v, cu_q, cu_k, causal, scale, lo=None):
+def _attn_fwd(q, k, v, cu_q, cu_k, causal, scale, lo=None, plan=None):
     """out and lse; lo (like out) gets what the rounding took from out."""
-    dt = _dtype("ogv.packed_attention", q, k, v)
+    dt = OGV_BF16 if q.dtype is torch.bfloat16 else OGV_F32
     Mq, heads, D = q.shape
-    out = torch.empty((Mq, heads, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((Mq, heads), dtype=torch.float32, device=q.device)
+    out = q.new_empty((Mq, heads, D))
+    lse = q.new_empty((Mq, heads), dtype=torch.float32)
     if Mq == 0:
         return out, lse
     B = cu_q.shape[0] - 1
@@ -121,8 +127,8 @@ def _attn_fwd(q, k, v, cu_q, cu_k, causal, scale, lo=None):
         if lo is not None:
             lo.zero_()
         return out.zero_(), lse.fill_(-math.inf)
-    d, ws, _ = _packed_desc(B, Mq, k.shape[0], heads, k.shape[1], D, causal, scale, dt, _strides(q), _strides(k), _strides(v),
-                            (heads * D, D))
+    d, ws, _ = plan or _packed_desc(B, Mq, k.shape[0], heads, k.shape[1], D, causal, scale, dt, _strides(q), _strides(k),
+                                    _strides(v), (heads * D, D))
     ws = _ws(ws, q)
     _launch(_lib.load().ogv_packed_attn_fwd, "ogv_packed_attn_fwd", q, _ptr(q), _ptr(k), _ptr(v), _ptr(cu_q), _ptr(cu_k),
             _ptr(out), _ptr(lo), _ptr(lse), _ptr(ws), d, dt)
@@ -173,7 +179,7 @@ class _PackedAttention(torch.autograd.Function):
 
 def _check_cu(what, cu):
     if cu.dtype is not torch.int32 or cu.ndim != 1 or cu.shape[0] < 1:
-        raise ValueError(f"{what}: int32 [sequences + 1] expected, got {cu.dtype} {tuple(cu.shape)}")
+        raise ValueError(f"{what}: row offsets must be int32 [sequences + 1], got {cu.dtype} {tuple(cu.shape)}")
     return cu if cu.is_contiguous() else cu.contiguous()
 
 
@@ -188,6 +194,25 @@ def _check_attention(what, D, heads, kv_heads, scale):
     return scale
 
 
+@functools.lru_cache(4096)
+def _attn_plan(what, q, qs, k, ks, v, vs, nq, nk, causal, scale, dt):
+    """What follows from shapes and strides: refusals; (scale, descriptor of a call without copies or None, group)."""
+    if len(q) != 3 or len(k) != 3 or len(v) != 3:
+        raise ValueError(f"{what}: q, k, v must be [rows, heads, head_dim]")
+    if k != v:
+        raise ValueError(f"{what}: k {tuple(k)} and v {tuple(v)} differ")
+    if q[2] != k[2]:
+        raise ValueError(f"{what}: head_dim of q ({q[2]}) and k ({k[2]}) differ")
+    scale = _check_attention(what, q[2], q[1], k[1], scale)
+    if nq != nk:
+        raise ValueError(f"{what}: cu_q has {nq} offsets, cu_k {nk}")
+    al, group, plan = 8 if dt == OGV_BF16 else 4, q[1] // k[1], None
+    if q[0] and nq > 1 and _addressable(q, qs, al, group) and _addressable(k, ks, al) and _addressable(v, vs, al):
+        plan = _packed_desc(nq - 1, q[0], k[0], q[1], k[1], q[2], causal, scale, dt, _row_head(q, qs), _row_head(k, ks),
+                            _row_head(v, vs), (q[1] * q[2], q[2]))
+    return scale, plan, group
+
+
 def packed_attention(q, k, v, cu_q, cu_k=None, causal=False, scale=None, return_lse=False):
     """softmax(scale q k^T) v inside each of the packed sequences.
 
@@ -200,21 +225,19 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal=False, scale=None, return_
     Returns out [rows, heads, D], with return_lse also the fp32 log-sum-exp [rows, heads] (no gradient).
     A non-finite value in v reaches its own sequence only, also where causal hides it."""
     what = "ogv.packed_attention"
-    if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
-        raise ValueError(f"{what}: q, k, v must be [rows, heads, head_dim]")
-    cu_k = cu_q if cu_k is None else cu_k
-    if k.shape != v.shape:
-        raise ValueError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
-    if q.shape[2] != k.shape[2]:
-        raise ValueError(f"{what}: head_dim of q ({q.shape[2]}) and k ({k.shape[2]}) differ")
-    scale = _check_attention(what, q.shape[2], q.shape[1], k.shape[1], scale)
-    _dtype(what, q, k, v)
-    cu_q, cu_k = _check_cu(f"{what}: cu_q", cu_q), _check_cu(f"{what}: cu_k", cu_k)
-    if cu_q.shape != cu_k.shape:
-        raise ValueError(f"{what}: cu_q has {cu_q.numel()} offsets, cu_k {cu_k.numel()}")
+    dt = _dtype(what, q, k, v)
+    causal = bool(causal)
+    cu_q = _check_cu(what, cu_q)
+    cu_k = cu_q if cu_k is None else _check_cu(what, cu_k)
+    scale, plan, group = _attn_plan(what, q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), cu_q.shape[0],
+                                    cu_k.shape[0], causal, scale, dt)
     _device(what, q, k, v, cu_q, cu_k)
-    fn = _PackedAttention.apply if _grad(q, k, v) else _attn_fwd
-    out, lse = fn(_heads3(q, q.shape[1] // k.shape[1]), _heads3(k), _heads3(v), cu_q, cu_k, bool(causal), scale)
+    if plan is None or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        q, k, v, plan = _heads3(q, group), _heads3(k), _heads3(v), None
+    if _grad(q, k, v):
+        out, lse = _PackedAttention.apply(q, k, v, cu_q, cu_k, causal, scale)
+    else:
+        out, lse = _attn_fwd(q, k, v, cu_q, cu_k, causal, scale, plan=plan)
     return (out, lse) if return_lse else out
 
 
@@ -232,22 +255,41 @@ def _rotary_desc(M, D, sections, theta, interleaved, inverse, pos_float, *tensor
     return ctypes.byref(d)
 
 
-def _rotate(xs, outs, positions, meta, inverse):
+def _rotate(xs, outs, positions, meta, inverse, desc=None):
     """Turn the one or two [M, heads, D] tensors xs into outs."""
     x = xs[0]
     if x.shape[0] == 0:
         return
-    d = _rotary_desc(x.shape[0], x.shape[2], *meta, inverse, positions.dtype is torch.float32,
-                     *((a.shape[1], _strides(a), _strides(b)) for a, b in zip(xs, outs)))
+    if desc is None:
+        desc = _rotary_desc(x.shape[0], x.shape[2], *meta, inverse, positions.dtype is torch.float32,
+                            *((a.shape[1], _strides(a), _strides(b)) for a, b in zip(xs, outs)))
     k, k_out = (xs[1], outs[1]) if len(xs) > 1 else (None, None)
-    _launch(_lib.load().ogv_axial_rotary, "ogv_axial_rotary", x, _ptr(x), _ptr(outs[0]), _ptr(k), _ptr(k_out), _ptr(positions), d,
-            _dtype("ogv.axial_rotary", *xs))
+    _launch(_lib.load().ogv_axial_rotary, "ogv_axial_rotary", x, _ptr(x), _ptr(outs[0]), _ptr(k), _ptr(k_out), _ptr(positions),
+            desc, OGV_BF16 if x.dtype is torch.bfloat16 else OGV_F32)
 
 
-def _rotate_new(positions, meta, *xs):
-    outs = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)
-    _rotate(xs, outs, positions, meta, False)
+def _rotate_new(positions, meta, *xs, desc=None):
+    outs = tuple([x.new_empty(x.shape) for x in xs])
+    _rotate(xs, outs, positions, meta, False, desc)
     return outs
+
+
+@functools.lru_cache(4096)
+def _rotary_plan(what, q, qs, k, ks, positions, pos_float, sections, theta, interleaved, al):
+    """What follows from shapes and strides: refusals; (meta, descriptor of a call without copies or None)."""
+    if len(q) != 3 or k is not None and len(k) != 3:
+        raise ValueError(f"{what}: q and k must be [rows, heads, head_dim]")
+    if not (q[1] > 0 and (k is None or k[1] > 0)):
+        raise ValueError(f"{what}: no heads")
+    if k is not None and (k[0] != q[0] or k[2] != q[2]):
+        raise ValueError(f"{what}: q {tuple(q)} and k {tuple(k)} differ in rows or head_dim")
+    meta = _rotary_meta(what, q[2], sections, theta, interleaved)
+    _positions_shape(what, positions, q[0], meta)
+    xs, desc = [(q, qs)] if k is None else [(q, qs), (k, ks)], None
+    if q[0] and all(_addressable(x, st, al) for x, st in xs):
+        desc = _rotary_desc(q[0], q[2], *meta, False, pos_float,
+                            *((x[1], _row_head(x, st), (x[1] * x[2], x[2])) for x, st in xs))
+    return meta, desc
 
 
 class _AxialRotary(torch.autograd.Function):
@@ -281,15 +323,17 @@ def _rotary_meta(what, D, sections, theta, interleaved):
     return sections, theta, bool(interleaved)
 
 
-def _check_rotary(what, D, positions, sections, theta, interleaved, rows):
-    meta = _rotary_meta(what, D, tuple(sections), theta, interleaved)
+def _positions_shape(what, shape, rows, meta):
+    if shape != (rows, len(meta[0])):
+        raise ValueError(f"{what}: positions [rows, axes] = [{rows}, {len(meta[0])}] expected, got {tuple(shape)}")
+
+
+def _check_positions(what, positions):
     if positions.dtype is not torch.int32 and positions.dtype is not torch.float32:
         raise TypeError(f"{what}: positions must be int32 or float32, got {positions.dtype}")
-    if positions.shape != (rows, len(meta[0])):
-        raise ValueError(f"{what}: positions [rows, axes] = [{rows}, {len(meta[0])}] expected, got {tuple(positions.shape)}")
     if positions.requires_grad:
         positions = positions.detach()
-    return positions if positions.is_contiguous() else positions.contiguous(), meta
+    return positions if positions.is_contiguous() else positions.contiguous()
 
 
 def axial_rotary(q, k, positions, sections, theta=10000.0, interleaved=False):
@@ -301,18 +345,18 @@ def axial_rotary(q, k, positions, sections, theta=10000.0, interleaved=False):
     by position * theta^(-j / n); pair p is the dims (p, p + P), or (2p, 2p + 1) with interleaved; dims from 2 P
     on pass unchanged.  Angles are reduced in 64 bits.  Positions get no gradient."""
     what = "ogv.axial_rotary"
-    if not (q.ndim == 3 and (k is None or k.ndim == 3)):
-        raise ValueError(f"{what}: q and k must be [rows, heads, head_dim]")
-    if not (q.shape[1] > 0 and (k is None or k.shape[1] > 0)):
-        raise ValueError(f"{what}: no heads")
-    if not (k is None or (k.shape[0] == q.shape[0] and k.shape[2] == q.shape[2])):
-        raise ValueError(f"{what}: q {tuple(q.shape)} and k {None if k is None else tuple(k.shape)} differ in rows or head_dim")
-    xs = (q,) if k is None else (q, k)
-    _dtype(what, *xs)
-    positions, meta = _check_rotary(what, q.shape[2], positions, sections, theta, interleaved, q.shape[0])
+    dt = _dtype(what, q, k)
+    if type(sections) is not tuple:
+        sections = tuple(sections)
+    positions = _check_positions(what, positions)
+    meta, desc = _rotary_plan(what, q.shape, q.stride(), None if k is None else k.shape, None if k is None else k.stride(),
+                              positions.shape, positions.dtype is torch.float32, sections, theta, interleaved,
+                              8 if dt == OGV_BF16 else 4)
     _device(what, q, k, positions)
-    fn = _AxialRotary.apply if _grad(*xs) else _rotate_new
-    outs = fn(positions, meta, *(_heads3(x) for x in xs))
+    if desc is None or (q.data_ptr() if k is None else q.data_ptr() | k.data_ptr()) & 15:
+        q, k, desc = _heads3(q), None if k is None else _heads3(k), None
+    xs = (q,) if k is None else (q, k)
+    outs = _AxialRotary.apply(positions, meta, *xs) if _grad(q, k) else _rotate_new(positions, meta, *xs, desc=desc)
     return outs[0] if k is None else outs
 
 
@@ -366,12 +410,13 @@ def rotary_attention_rows(qkv, cu, heads, kv_heads=None, positions=None, section
     D = qkv.shape[1] // (heads + 2 * kv_heads)
     scale = _check_attention(what, D, heads, kv_heads, scale)
     _dtype(what, qkv)
-    cu = _check_cu(f"{what}: cu", cu)
+    cu = _check_cu(what, cu)
     if not ((positions is None) == (sections is None)):
         raise ValueError(f"{what}: positions and sections belong together")
     rot = None
     if positions is not None:
-        positions, rot = _check_rotary(what, D, positions, sections, theta, interleaved, qkv.shape[0])
+        positions, rot = _check_positions(what, positions), _rotary_meta(what, D, tuple(sections), theta, interleaved)
+        _positions_shape(what, positions.shape, qkv.shape[0], rot)
     _device(what, qkv, cu, positions)
     al = 16 // qkv.element_size()
     if qkv.stride(1) != 1 or qkv.stride(0) % al or qkv.data_ptr() % 16:
