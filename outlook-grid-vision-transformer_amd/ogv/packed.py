@@ -435,13 +435,13 @@ def _norm_desc(M, C, post, pre, samples, rps, alpha, post_eps, pre_eps, dt):
     return d, _lib.load().ogv_gated_norm_bwd_ws_bytes(d, dt)
 
 
-def _norm_fwd(f, x, gate, rs, post_w, post_b, pre_w, pre_b, meta, stats=None):
-    dt = _dtype("ogv.gated_residual_norm", f, x)
+def _norm_fwd(f, x, gate, rs, post_w, post_b, pre_w, pre_b, meta, stats=None, desc=None):
+    dt = OGV_BF16 if f.dtype is torch.bfloat16 else OGV_F32
     y = torch.empty_like(f)
     h = torch.empty_like(f) if meta[1] else None
     if f.shape[0]:
         _launch(_lib.load().ogv_gated_norm_fwd, "ogv_gated_norm_fwd", f, _ptr(f), _ptr(x), _ptr(gate), _ptr(rs), _ptr(post_w),
-                _ptr(post_b), _ptr(pre_w), _ptr(pre_b), _ptr(y), _ptr(h), _ptr(stats), _norm_desc(*f.shape, *meta, dt)[0], dt)
+                _ptr(post_b), _ptr(pre_w), _ptr(pre_b), _ptr(y), _ptr(h), _ptr(stats), desc or _norm_desc(*f.shape, *meta, dt)[0], dt)
     return y if h is None else (y, h)
 
 
@@ -492,6 +492,54 @@ class _GatedNorm(torch.autograd.Function):
                 None if pre_w is None else w1, None if pre_b is None else b1, None)
 
 
+def _shape(t):
+    return None if t is None else t.shape
+
+
+def _f32c(t):
+    """A parameter as contiguous fp32."""
+    if t is None:
+        return None
+    t = f32(t)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+@functools.lru_cache(4096)
+def _norm_plan(what, branch, residual, gate, factors, rps, post_norm, post_w, post_b, pre_norm, pre_w, pre_b, alpha, post_eps,
+               pre_eps, dt):
+    """What follows from shapes: refusals; (meta, descriptor)."""
+    if len(branch) != 2 or branch != residual:
+        raise ValueError(f"{what}: branch {tuple(branch)} and residual {tuple(residual)} must be equal [rows, channels]")
+    M, C = branch
+    if post_norm not in NORMS or pre_norm not in NORMS:
+        raise ValueError(f"{what}: norms are 'layer', 'rms' or None, got {post_norm!r}, {pre_norm!r}")
+    if not 1 <= C <= 8192:
+        raise ValueError(f"{what}: {C} channels unsupported (1 to 8192)")
+    post, pre = NORMS[post_norm], NORMS[pre_norm]
+    if not post and not (post_w is None and post_b is None):
+        raise ValueError(f"{what}: weights for an absent post_norm")
+    if not pre and not (pre_w is None and pre_b is None):
+        raise ValueError(f"{what}: weights for an absent pre_norm")
+    for name, p in (("post_weight", post_w), ("post_bias", post_b), ("pre_weight", pre_w), ("pre_bias", pre_b)):
+        if p is not None and p != (C,):
+            raise ValueError(f"{what}: {name} must be [{C}]")
+    samples = 1
+    if gate is not None:
+        if len(gate) not in (1, 2) or gate[-1] != C:
+            raise ValueError(f"{what}: gate must be [{C}] or [samples, {C}], got {tuple(gate)}")
+        if len(gate) == 2:
+            samples = gate[0]
+            if samples < 1 or M % samples:
+                raise ValueError(f"{what}: {M} rows do not divide into {samples} samples")
+    rps = int(rps)
+    if rps < 1:
+        raise ValueError(f"{what}: rps must be >= 1")
+    if factors is not None and factors * rps < M:
+        raise ValueError(f"{what}: row_scale has {factors} factors of {rps} rows for {M} rows")
+    meta = (post, pre, samples, rps, alpha, post_eps, pre_eps)
+    return meta, _norm_desc(M, C, *meta, dt)[0] if M else None
+
+
 def gated_residual_norm(branch, residual, gate=None, row_scale=None, rps=1, alpha=1.0, post_norm=None, post_weight=None,
                         post_bias=None, pre_norm="layer", pre_weight=None, pre_bias=None, post_eps=1e-5, pre_eps=1e-5):
     """The end of a residual half-block and the norm that begins the next one:
@@ -503,42 +551,20 @@ def gated_residual_norm(branch, residual, gate=None, row_scale=None, rps=1, alph
     each.  row_scale fp32, one factor per rps rows (DropPath's; it gets no gradient).
     Returns (y, h), or y alone without a pre_norm.  h comes from y before its rounding.  C <= 8192."""
     what = "ogv.gated_residual_norm"
-    if not (branch.ndim == 2 and branch.shape == residual.shape):
-        raise ValueError(f"{what}: branch {tuple(branch.shape)} and residual "
-                         f"{tuple(residual.shape)} must be equal [rows, channels]")
-    M, C = branch.shape
-    if not (post_norm in NORMS and pre_norm in NORMS):
-        raise ValueError(f"{what}: norms are 'layer', 'rms' or None, got {post_norm!r}, {pre_norm!r}")
-    if not (1 <= C <= 8192):
-        raise ValueError(f"{what}: {C} channels unsupported (1 to 8192)")
-    _dtype(what, branch, residual)
-    post, pre = NORMS[post_norm], NORMS[pre_norm]
-    if not (post or (post_weight is None and post_bias is None)):
-        raise ValueError(f"{what}: weights for an absent post_norm")
-    if not (pre or (pre_weight is None and pre_bias is None)):
-        raise ValueError(f"{what}: weights for an absent pre_norm")
-    params = []
-    for name, p in (("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight), ("pre_bias", pre_bias)):
-        if not (p is None or p.shape == (C,)):
-            raise ValueError(f"{what}: {name} must be [{C}]")
-        params.append(None if p is None else f32(p).contiguous())
-    samples = 1
-    if gate is not None:
-        if not (gate.ndim in (1, 2) and gate.shape[-1] == C):
-            raise ValueError(f"{what}: gate must be [{C}] or [samples, {C}], got {tuple(gate.shape)}")
-        if gate.ndim == 2:
-            samples = gate.shape[0]
-            if not (samples >= 1 and M % samples == 0):
-                raise ValueError(f"{what}: {M} rows do not divide into {samples} samples")
-        gate = f32(gate).contiguous()
-    rps = int(rps)
-    if not (rps >= 1):
-        raise ValueError(f"{what}: rps must be >= 1")
+    dt = _dtype(what, branch, residual)
+    meta, desc = _norm_plan(what, branch.shape, residual.shape, None if gate is None else gate.shape,
+                            None if row_scale is None else row_scale.numel(), rps, post_norm, _shape(post_weight),
+                            _shape(post_bias), pre_norm, _shape(pre_weight), _shape(pre_bias), float(alpha), float(post_eps),
+                            float(pre_eps), dt)
     if row_scale is not None:
-        if not (row_scale.numel() * rps >= M):
-            raise ValueError(f"{what}: row_scale has {row_scale.numel()} factors of {rps} rows for {M} rows")
-        row_scale = row_scale.detach().float().reshape(-1).contiguous()
+        row_scale = _f32c(row_scale.detach().reshape(-1))
+    gate = _f32c(gate)
+    params = _f32c(post_weight), _f32c(post_bias), _f32c(pre_weight), _f32c(pre_bias)
     _device(what, branch, residual, gate, row_scale, *params)
-    meta = (post, pre, samples, rps, float(alpha), float(post_eps), float(pre_eps))
-    fn = _GatedNorm.apply if _grad(branch, residual, gate, *params) else _norm_fwd
-    return fn(branch.contiguous(), residual.contiguous(), gate, row_scale, *params, meta)
+    if not branch.is_contiguous():
+        branch = branch.contiguous()
+    if not residual.is_contiguous():
+        residual = residual.contiguous()
+    if _grad(branch, residual, gate, *params):
+        return _GatedNorm.apply(branch, residual, gate, row_scale, *params, meta)
+    return _norm_fwd(branch, residual, gate, row_scale, *params, meta, desc=desc)
