@@ -35,7 +35,7 @@ __device__ __forceinline__ void dq_tile(const char* Ks, const char* Vs, const Ch
                                         float lse2, float delta, int lane) {
   constexpr int KK = Frag<T, D>::KK, RB = Frag<T, D>::RB;
   const int hf = lane >> 5, c = lane & 31;
-#pragma unroll 1
+#pragma unroll (D <= 64 ? NB : 1)   // (larger heads have no registers for two blocks at once)
   for (int nb = 0; nb < NB; ++nb) {
     f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
@@ -144,7 +144,7 @@ __device__ __forceinline__ void dkv_tile(const char* Qs, const char* Gs, const f
                                          int off, int j, int jmax, const PackedArgs& a, float c2, int lane) {
   constexpr int KK = Frag<T, D>::KK, RB = Frag<T, D>::RB;
   const int hf = lane >> 5, c = lane & 31;
-#pragma unroll 1
+#pragma unroll (D <= 64 ? NB : 1)   // (larger heads have no registers for two blocks at once)
   for (int nb = 0; nb < NB; ++nb) {
     f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
@@ -178,7 +178,7 @@ __device__ __forceinline__ void dkv_tile(const char* Qs, const char* Gs, const f
 // that see them.  Heads of 96 and 128 keep V in LDS instead of registers: that leaves two waves to a SIMD (at one,
 // nothing covers the exponentials and the LDS reads).  One piece writes dk, dv; several write fp32 partial sums.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dkv_kernel(const PackedArgs a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && (NW > 1 || D < 128) ? 2 : 1) void packed_dkv_kernel(const PackedArgs a) {
   using F = Frag<T, D>;
   constexpr bool VL = sizeof(T) == 2 && D >= 96;
   constexpr int BM = 32 * NW, BN = sizeof(T) == 2 && NW > 1 && !VL ? 64 : 32, NB = BN / 32;   // BM keys, BN rows per step
