@@ -209,25 +209,33 @@ __device__ __forceinline__ Chunk pack8(const f32x16& x, int s) {
 
 // acc[db] += X^T . Y for one 32-row block of the LDS tile: X is rows row0 .. row0 + 31 of the tile, y the
 // C tile whose rows are the same 32 rows, acc[db] the dims 32 * db .. + 31 (rows) of y's columns.
-template <typename T, int D>
+// AHEAD: each LDS read is issued before the product in front of it (the compiler, short of registers, puts it behind).
+template <typename T, int D, bool AHEAD = false>
 __device__ __forceinline__ void accum_xt(const char* tile, int row0, const f32x16& y, f32x16 (&acc)[D / 32], int lane) {
   constexpr int RB = Frag<T, D>::RB;
   const int hf = lane >> 5;
   if constexpr (sizeof(T) == 2) {
     const int fr = lane & 15, part = (lane >> 4) & 1;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const Chunk yb = pack8(y, s);
+    union X { s16x4 p[2]; bf16x8 h; };
+    auto read = [&](int s, int db) {
       const int row = row0 + 16 * s + 4 * hf + (fr >> 2);
       const int sw0 = swz<RB>(row), sw1 = swz<RB>(row + 8);
+      const int ch = db * 4 + part * 2 + ((fr >> 1) & 1), sub = (fr & 1) * 8;
+      X a;
+      a.p[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_t*)(tile + row * RB + ((ch ^ sw0) << 4) + sub));
+      a.p[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_t*)(tile + (row + 8) * RB + ((ch ^ sw1) << 4) + sub));
+      return a;
+    };
+    const Chunk yb[2] = {pack8(y, 0), pack8(y, 1)};
+    X a = read(0, 0);
 #pragma unroll
-      for (int db = 0; db < D / 32; ++db) {
-        const int ch = db * 4 + part * 2 + ((fr >> 1) & 1), sub = (fr & 1) * 8;
-        union { s16x4 p[2]; bf16x8 h; } a;
-        a.p[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_t*)(tile + row * RB + ((ch ^ sw0) << 4) + sub));
-        a.p[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_t*)(tile + (row + 8) * RB + ((ch ^ sw1) << 4) + sub));
-        acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, yb.h, acc[db], 0, 0, 0);
-      }
+    for (int i = 0; i < 2 * (D / 32); ++i) {
+      const int s = i / (D / 32), db = i % (D / 32);
+      const X n = i + 1 < 2 * (D / 32) ? read((i + 1) / (D / 32), (i + 1) % (D / 32)) : a;
+      if (AHEAD) __builtin_amdgcn_sched_barrier(0);
+      acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, yb[s].h, acc[db], 0, 0, 0);
+      if (AHEAD) __builtin_amdgcn_sched_barrier(0);
+      a = n;
     }
   } else {
     const int c = lane & 31;

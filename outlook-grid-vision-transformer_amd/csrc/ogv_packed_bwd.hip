@@ -35,7 +35,8 @@ __device__ __forceinline__ void dq_tile(const char* Ks, const char* Vs, const Ch
                                         float lse2, float delta, int lane) {
   constexpr int KK = Frag<T, D>::KK, RB = Frag<T, D>::RB;
   const int hf = lane >> 5, c = lane & 31;
-#pragma unroll (D <= 64 ? NB : 1)   // (larger heads have no registers for two blocks at once)
+  constexpr int AT_ONCE = D <= 64 ? NB : 1;   // larger heads have no registers for two blocks at once
+#pragma unroll AT_ONCE
   for (int nb = 0; nb < NB; ++nb) {
     f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
@@ -137,20 +138,34 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dq_ker
   store_cols<T, D>((T*)a.dq + (long)(sq.start + pos) * a.rdq + (long)(h * a.G + hg) * a.hsdq, dq, a.scale, a.D, hf, r < store_rows);
 }
 
-// 32 * NB rows of dk / dv: scores and dp with columns = keys, dV^T += dO^T P, dK^T += Q^T dS
+// 32 * NB rows of dk / dv: scores and dp with columns = keys, dV^T += dO^T P, dK^T += Q^T dS.  With V in LDS (VL) nearly all
+// registers are taken and the compiler would put each LDS read right before its product; read one product ahead instead
+// (long causal streams, D = 128: the step 555 -> 535 us; heads of 64, and dq, have the registers and gain nothing).
 template <typename T, int D, int NB, bool VL>
 __device__ __forceinline__ void dkv_tile(const char* Qs, const char* Gs, const float2* St, const Chunk (&kf)[Frag<T, D>::KK],
                                          const Chunk (&vf)[VL ? 1 : Frag<T, D>::KK], const char* Vs, f32x16 (&dk)[D / 32], f32x16 (&dv)[D / 32], int rt,
                                          int off, int j, int jmax, const PackedArgs& a, float c2, int lane) {
   constexpr int KK = Frag<T, D>::KK, RB = Frag<T, D>::RB;
   const int hf = lane >> 5, c = lane & 31;
-#pragma unroll (D <= 64 ? NB : 1)   // (larger heads have no registers for two blocks at once)
+  constexpr int AT_ONCE = D <= 64 ? NB : 1;   // larger heads have no registers for two blocks at once
+#pragma unroll AT_ONCE
   for (int nb = 0; nb < NB; ++nb) {
     f32x16 s = f32x16{}, dp = f32x16{};
+    Chunk qa = lds_chunk<RB>(Qs, nb * 32 + c, hf), ga = lds_chunk<RB>(Gs, nb * 32 + c, hf), va;
+    if (VL) va = lds_chunk<RB>(Vs, c, hf);
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
-      mfma_step<T>(lds_chunk<RB>(Qs, nb * 32 + c, 2 * kk + hf), kf[kk], s);
-      mfma_step<T>(lds_chunk<RB>(Gs, nb * 32 + c, 2 * kk + hf), VL ? lds_chunk<RB>(Vs, c, 2 * kk + hf) : vf[VL ? 0 : kk], dp);
+      const int nx = 2 * (kk + 1) + hf;
+      Chunk qn = qa, gn = ga, vn = va;
+      if (kk + 1 < KK) {
+        qn = lds_chunk<RB>(Qs, nb * 32 + c, nx), gn = lds_chunk<RB>(Gs, nb * 32 + c, nx);
+        if (VL) vn = lds_chunk<RB>(Vs, c, nx);
+      }
+      if (VL) __builtin_amdgcn_sched_barrier(0);
+      mfma_step<T>(qa, kf[kk], s);
+      mfma_step<T>(ga, VL ? va : vf[VL ? 0 : kk], dp);
+      if (VL) __builtin_amdgcn_sched_barrier(0);
+      qa = qn, ga = gn, va = vn;
     }
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
@@ -169,8 +184,8 @@ __device__ __forceinline__ void dkv_tile(const char* Qs, const char* Gs, const f
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) dp[i] *= s[i];
-    accum_xt<T, D>(Gs, nb * 32, s, dv, lane);
-    accum_xt<T, D>(Qs, nb * 32, dp, dk, lane);
+    accum_xt<T, D, VL>(Gs, nb * 32, s, dv, lane);
+    accum_xt<T, D, VL>(Qs, nb * 32, dp, dk, lane);
   }
 }
 
@@ -326,8 +341,9 @@ struct BwdPlan {
 
 // Waves per workgroup as in the forward.  The rows of dk / dv are split while the key tiles would not fill the 256 CUs
 // twice, into 1024 workgroups or a few more (two to a CU, twice: under the causal mask the first tile has twice the
-// average work; long causal streams, D = 128: 580 us for the step with 768, 549 with 1024, 569 with 1536).  A piece costs 16 bytes of partial sums
-// per key, head and dim, so it has at least 512 rows on average, 32 in fp32, whose products run at a sixteenth of the rate.
+// average work; long causal streams, D = 128: with 768 the step takes 1.06, with 1536 1.04 times as long).  A piece costs
+// 16 bytes of partial sums per key, head and dim, so it has at least 512 rows on average, 32 in fp32, whose products run
+// at a sixteenth of the rate.
 static BwdPlan bwd_plan(const ogv_packed_desc* d, ogv_dtype dt) {
   BwdPlan p;
   const long rows = (long)d->Mq * (d->heads / d->kv_heads);
