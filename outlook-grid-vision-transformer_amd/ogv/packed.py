@@ -26,6 +26,7 @@ NORMS = {None: 0, "none": 0, "layer": 1, "rms": 2}
 
 # Small calls are bound by the host, so what depends on sizes alone (the C-ABI's descriptors and workspace sizes) is
 # looked up by value, the device is only switched where it differs, and calls without gradients skip autograd.
+# What a caller passes as a number becomes one first: a tensor as a key would stand for its identity, not its value.
 
 
 def _dtype(what, first, *ts):
@@ -48,6 +49,13 @@ def _device(what, first, *ts):
                                    f"this framework has no CPU execution path")
             if t.get_device() != dev:
                 raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+
+
+def _rows32(what, *rows):
+    """The C-ABI counts rows in 32 bits."""
+    for m in rows:
+        if m >= 1 << 31:
+            raise ValueError(f"{what}: too many rows ({m})")
 
 
 def _grad(*ts):
@@ -106,6 +114,7 @@ def _strides(t):
 @functools.lru_cache(4096)
 def _packed_desc(B, Mq, Mk, heads, kv_heads, D, causal, scale, dt, *strides):
     """(descriptor, forward workspace bytes, backward workspace bytes)."""
+    _rows32("ogv.packed_attention", Mq, Mk, B)
     d = PackedDesc(B=B, Mq=Mq, Mk=Mk, heads=heads, kv_heads=kv_heads, D=D, causal=causal, scale=scale)
     for i, (row, head) in enumerate(strides):
         d.row[i], d.head[i] = row, head
@@ -226,7 +235,7 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal=False, scale=None, return_
     A non-finite value in v reaches its own sequence only, also where causal hides it."""
     what = "ogv.packed_attention"
     dt = _dtype(what, q, k, v)
-    causal = bool(causal)
+    causal, scale = bool(causal), None if scale is None else float(scale)
     cu_q = _check_cu(what, cu_q)
     cu_k = cu_q if cu_k is None else _check_cu(what, cu_k)
     scale, plan, group = _attn_plan(what, q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), cu_q.shape[0],
@@ -246,6 +255,7 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal=False, scale=None, return_
 # ------------------------------------------------------------------------------------------------
 @functools.lru_cache(4096)
 def _rotary_desc(M, D, sections, theta, interleaved, inverse, pos_float, *tensors):
+    _rows32("ogv.axial_rotary", M)
     d = RotaryDesc(M=M, D=D, axes=len(sections), interleaved=interleaved, inverse=inverse, pos_float=pos_float, theta=theta)
     for i, n in enumerate(sections):
         d.pairs[i] = n
@@ -311,16 +321,14 @@ class _AxialRotary(torch.autograd.Function):
 
 @functools.lru_cache(1024)
 def _rotary_meta(what, D, sections, theta, interleaved):
-    sections = tuple(int(n) for n in sections)
     if not (1 <= len(sections) <= 4 and all(n > 0 for n in sections)):
         raise ValueError(f"{what}: sections must be 1 to 4 positive pair counts, got {sections}")
     if not (D % 2 == 0 and D <= 128 and 2 * sum(sections) <= D):
         raise ValueError(f"{what}: {sum(sections)} pairs need an even head_dim of at "
                          f"least {2 * sum(sections)} (and at most 128), got {D}")
-    theta = float(theta)
     if not 0.0 < theta < math.inf:
         raise ValueError(f"{what}: theta must be positive and finite, got {theta}")
-    return sections, theta, bool(interleaved)
+    return sections, theta, interleaved
 
 
 def _positions_shape(what, shape, rows, meta):
@@ -346,11 +354,10 @@ def axial_rotary(q, k, positions, sections, theta=10000.0, interleaved=False):
     on pass unchanged.  Angles are reduced in 64 bits.  Positions get no gradient."""
     what = "ogv.axial_rotary"
     dt = _dtype(what, q, k)
-    if type(sections) is not tuple:
-        sections = tuple(sections)
+    sections = tuple([int(n) for n in sections])
     positions = _check_positions(what, positions)
     meta, desc = _rotary_plan(what, q.shape, q.stride(), None if k is None else k.shape, None if k is None else k.stride(),
-                              positions.shape, positions.dtype is torch.float32, sections, theta, interleaved,
+                              positions.shape, positions.dtype is torch.float32, sections, float(theta), bool(interleaved),
                               8 if dt == OGV_BF16 else 4)
     _device(what, q, k, positions)
     if desc is None or (q.data_ptr() if k is None else q.data_ptr() | k.data_ptr()) & 15:
@@ -415,11 +422,12 @@ def rotary_attention_rows(qkv, cu, heads, kv_heads=None, positions=None, section
         raise ValueError(f"{what}: positions and sections belong together")
     rot = None
     if positions is not None:
-        positions, rot = _check_positions(what, positions), _rotary_meta(what, D, tuple(sections), theta, interleaved)
+        positions = _check_positions(what, positions)
+        rot = _rotary_meta(what, D, tuple([int(n) for n in sections]), float(theta), bool(interleaved))
         _positions_shape(what, positions.shape, qkv.shape[0], rot)
     _device(what, qkv, cu, positions)
     al = 16 // qkv.element_size()
-    if qkv.stride(1) != 1 or qkv.stride(0) % al or qkv.data_ptr() % 16:
+    if qkv.stride(1) != 1 or qkv.stride(0) % al or qkv.stride(0) >= 1 << 24 or qkv.data_ptr() % 16:
         qkv = qkv.clone(memory_format=torch.contiguous_format)
     return _RotaryAttentionRows.apply(qkv, cu, positions, rot, int(heads), kv_heads, bool(causal), scale)
 
@@ -430,6 +438,7 @@ def rotary_attention_rows(qkv, cu, heads, kv_heads=None, positions=None, section
 @functools.lru_cache(4096)
 def _norm_desc(M, C, post, pre, samples, rps, alpha, post_eps, pre_eps, dt):
     """(descriptor, backward workspace bytes)."""
+    _rows32("ogv.gated_residual_norm", M)
     d = ctypes.byref(GatedNormDesc(M=M, C=C, post=post, pre=pre, samples=samples, rps=rps, alpha=alpha, post_eps=post_eps,
                                    pre_eps=pre_eps))
     return d, _lib.load().ogv_gated_norm_bwd_ws_bytes(d, dt)
@@ -531,12 +540,11 @@ def _norm_plan(what, branch, residual, gate, factors, rps, post_norm, post_w, po
             samples = gate[0]
             if samples < 1 or M % samples:
                 raise ValueError(f"{what}: {M} rows do not divide into {samples} samples")
-    rps = int(rps)
     if rps < 1:
         raise ValueError(f"{what}: rps must be >= 1")
     if factors is not None and factors * rps < M:
         raise ValueError(f"{what}: row_scale has {factors} factors of {rps} rows for {M} rows")
-    meta = (post, pre, samples, rps, alpha, post_eps, pre_eps)
+    meta = (post, pre, samples, max(1, min(rps, M)), alpha, post_eps, pre_eps)
     return meta, _norm_desc(M, C, *meta, dt)[0] if M else None
 
 
@@ -553,7 +561,7 @@ def gated_residual_norm(branch, residual, gate=None, row_scale=None, rps=1, alph
     what = "ogv.gated_residual_norm"
     dt = _dtype(what, branch, residual)
     meta, desc = _norm_plan(what, branch.shape, residual.shape, None if gate is None else gate.shape,
-                            None if row_scale is None else row_scale.numel(), rps, post_norm, _shape(post_weight),
+                            None if row_scale is None else row_scale.numel(), int(rps), post_norm, _shape(post_weight),
                             _shape(post_bias), pre_norm, _shape(pre_weight), _shape(pre_bias), float(alpha), float(post_eps),
                             float(pre_eps), dt)
     if row_scale is not None:

@@ -200,3 +200,51 @@ def test_oracle_forms_against_differences():
     y, _ = R.rotary(x, pos, (2, 3), 100.0, True)
     z, _ = R.rotary(y, pos, (2, 3), 100.0, True, inverse=True)
     assert (z - x.double()).abs().max() < 1e-12
+
+
+def test_numbers_given_as_tensors_count_by_their_value():
+    """What is looked up by value must not be found again by the identity of a tensor whose value has changed."""
+    from ogv.packed import axial_rotary, gated_residual_norm, packed_attention
+    cpu = pytest.raises(RuntimeError, match="HIP device")   # past every check of the arguments
+    scale = torch.tensor(0.25)
+    with cpu:
+        packed_attention(**_attn(scale=scale))
+    scale.neg_()
+    with pytest.raises(ValueError, match="scale"):
+        packed_attention(**_attn(scale=scale))
+    theta, n = torch.tensor(1e4), torch.tensor(4)
+    rot = dict(q=torch.zeros(5, 3, 16), k=None, positions=torch.zeros(5, 2, dtype=torch.int32))
+    with cpu:
+        axial_rotary(**rot, sections=(n, 4), theta=theta)
+    theta.neg_()
+    with pytest.raises(ValueError, match="theta"):
+        axial_rotary(**rot, sections=(n, 4), theta=theta)
+    theta.neg_()
+    n.fill_(5)
+    with pytest.raises(ValueError, match="pairs"):
+        axial_rotary(**rot, sections=(n, 4), theta=theta)
+    x, rs, rps = torch.zeros(4, 8), torch.ones(2), torch.tensor(2)
+    with cpu:
+        gated_residual_norm(x, x, row_scale=rs, rps=rps)
+    rps.fill_(1)
+    with pytest.raises(ValueError, match="factors"):
+        gated_residual_norm(x, x, row_scale=rs, rps=rps)
+
+
+def test_rows_beyond_32_bits_are_refused():
+    """Row counts are 32-bit in the C-ABI: a larger one is an error, never a smaller call."""
+    from ogv.packed import axial_rotary, gated_residual_norm, packed_attention
+    big = (1 << 32) + 5
+
+    few = _attn()
+    rows = torch.empty(big, 2, 16, device="meta")
+    for more in (dict(q=torch.empty(big, 4, 16, device="meta")), dict(k=rows, v=rows)):
+        with pytest.raises(ValueError, match="too many rows"):
+            packed_attention(**{**few, **more})
+    with pytest.raises(ValueError, match="too many rows"):
+        axial_rotary(rows, None, torch.empty(big, 1, dtype=torch.int32, device="meta"), (8,))
+    x = torch.empty(big, 8, device="meta")
+    with pytest.raises(ValueError, match="too many rows"):
+        gated_residual_norm(x, x)
+    with pytest.raises(RuntimeError, match="HIP device"):   # more rows per factor than rows: one factor, nothing to refuse
+        gated_residual_norm(torch.zeros(4, 8), torch.zeros(4, 8), row_scale=torch.ones(1), rps=big)
