@@ -226,16 +226,25 @@ __device__ __forceinline__ void accum_xt(const char* tile, int row0, const f32x1
       a.p[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_t*)(tile + (row + 8) * RB + ((ch ^ sw1) << 4) + sub));
       return a;
     };
-    const Chunk yb[2] = {pack8(y, 0), pack8(y, 1)};
-    X a = read(0, 0);
+    if constexpr (AHEAD) {
+      const Chunk yb[2] = {pack8(y, 0), pack8(y, 1)};
+      X a = read(0, 0);
 #pragma unroll
-    for (int i = 0; i < 2 * (D / 32); ++i) {
-      const int s = i / (D / 32), db = i % (D / 32);
-      const X n = i + 1 < 2 * (D / 32) ? read((i + 1) / (D / 32), (i + 1) % (D / 32)) : a;
-      if (AHEAD) __builtin_amdgcn_sched_barrier(0);
-      acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, yb[s].h, acc[db], 0, 0, 0);
-      if (AHEAD) __builtin_amdgcn_sched_barrier(0);
-      a = n;
+      for (int i = 0; i < 2 * (D / 32); ++i) {
+        const int db = i % (D / 32);
+        const X n = i + 1 < 2 * (D / 32) ? read((i + 1) / (D / 32), (i + 1) % (D / 32)) : a;
+        __builtin_amdgcn_sched_barrier(0);
+        acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, yb[i / (D / 32)].h, acc[db], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        a = n;
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const Chunk yb = pack8(y, s);
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read(s, db).h, yb.h, acc[db], 0, 0, 0);
+      }
     }
   } else {
     const int c = lane & 31;

@@ -177,10 +177,8 @@ __device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* tiles, int h
       f32x16 next[NB];
       fwd_scores<T, D, NB>(tiles + (at ^ TB), qf, next, lane);
       fwd_weights<NB>(s, l, c2, mu);
-      // (V read ahead of each product: 48 images, heads of 64: 102 -> 98 us, long causal streams 413 -> 411; the whole
-      // tile in one run of products, one to three reads ahead, is slower: 107 and 434 to 442)
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) accum_xt<T, D, true>(tiles + 2 * TB + at, nb * 32, s[nb], o, lane);
+      for (int nb = 0; nb < NB; ++nb) accum_xt<T, D>(tiles + 2 * TB + at, nb * 32, s[nb], o, lane);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) s[nb] = next[nb];
     }
@@ -188,7 +186,7 @@ __device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* tiles, int h
     tiles_ready();
     fwd_weights<NB>(s, l, c2, mu);
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) accum_xt<T, D, true>(tiles + 2 * TB + at, nb * 32, s[nb], o, lane);
+    for (int nb = 0; nb < NB; ++nb) accum_xt<T, D>(tiles + 2 * TB + at, nb * 32, s[nb], o, lane);
   }
 
   l = pair_sum(l);
