@@ -12,7 +12,7 @@
 // than dS's rounding (dq of short sequences: 0.0032 off in 2-norm instead of 0.0024).
 //
 // Measured on one MI355X: D = 128, causal, 16 heads on 4, sequences of 4096 and 2451 (327 GFLOP with the forward): dq 177 us
-// (791 TFLOP/s of its three products), dk / dv 289 us (647, four products) and 23 us to add its row pieces.  Both are
+// (791 TFLOP/s of its three products), dk / dv 259 us (722, four products) and 23 us to add its row pieces.  Both are
 // bound by the matrix instructions and the LDS reads that feed them (24 and 40 KB a 32x32 block of scores).  D = 64, 64
 // images of 49 to 784 tokens, 6 heads: dq 56 us and dk / dv 59 us, of which 22 and 16 are the workgroups' ends (rows read
 // and written); 5 tiles a workgroup do not hide the rest.
