@@ -206,7 +206,8 @@ int ogv_layernorm_bwd(const void* dy, const void* x, const float* gamma, const f
  *   q, out [Mq][heads][D], k, v [Mk][kv_heads][D] with the given row and head strides (elements, multiples of
  *   16 bytes; the last dim is contiguous, pointers 16-B aligned); lse fp32 [Mq][heads].
  *   Sequence b: queries cu_q[b] .. cu_q[b + 1] - 1, keys cu_k[b] .. cu_k[b + 1] - 1 (int32 [B + 1] on the device,
- *   not decreasing; the first offset is taken as 0, all are clamped to [0, M]).  Any length may be 0.
+ *   not decreasing; the first offset is taken as 0, all are clamped to [0, M]).  Any length may be 0.  Offsets that
+ *   decrease are the caller's error: nothing outside the tensors is read or written, what the results hold is unspecified.
  *   causal: key j of a sequence is seen by its query i where j <= i + keys - queries.
  *   A row that sees no key, and a row behind the last sequence: out 0, lse -inf, gradients 0.
  * out_lo, like out (NULL: not wanted; bf16 only): what the rounding took from out, for a backward.

@@ -67,11 +67,11 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_dq_ker
   int h, t;
   if (!head_tile(a.d, a.hkv, a.tiles, h, t)) return;
   if (a.D < D) clear_tiles<4 * TB, NW * 64>(tiles, tid);
-  const Seq sq = find_tile(a.cu_q, a.cu_k, a.B, a.Mq, a.Mk, a.G, BM, a.tiles - 1 - t, lane);
+  Seq sq;
+  if (!find_tile(a.cu_q, a.cu_k, a.B, a.Mq, a.Mk, a.G, BM, a.tiles - 1 - t, lane, sq)) return;
   const int k0 = sq.start2, lk = sq.len2;
   const int rows = sq.len * a.G, r0 = sq.tile * BM;
   const int store_rows = sq.b == a.B - 1 ? (a.Mq - sq.start) * a.G : rows;
-  if (r0 >= store_rows) return;
   const int off = lk - sq.len;
   int kend = r0 < rows ? lk : 0;
   if (a.causal && kend) kend = max(0, min(lk, group_div(min(r0 + BM, rows) - 1, a.G, a.gmagic) + off + 1));
@@ -210,11 +210,11 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && (NW > 1 || D < 128) ? 2 
   if (a.D < D) clear_tiles<4 * TB, NT>(tiles, tid);
   if (VL && a.D < D) clear_tiles<sizeof(Vl), NT>(Vl, tid);
   const int split = t % a.nsplit;
-  const Seq sk = find_tile(a.cu_k, a.cu_q, a.B, a.Mk, a.Mq, 1, BM, t / a.nsplit, lane);
+  Seq sk;
+  if (!find_tile(a.cu_k, a.cu_q, a.B, a.Mk, a.Mq, 1, BM, t / a.nsplit, lane, sk)) return;
   const int q0 = sk.start2, lq = sk.len2;
   const int j0 = sk.tile * BM, off = sk.len - lq, rows = lq * a.G;
   const int store_keys = sk.b == a.B - 1 ? a.Mk - sk.start : sk.len;
-  if (j0 >= store_keys) return;
   int rend = j0 < sk.len ? rows : 0, rbeg = 0;
   if (a.causal) rbeg = (int)(min((long)rend, (long)max(0, j0 - off) * a.G) / BN) * BN;   // rows that see key j0 or later
   if (a.nsplit > 1) {

@@ -106,7 +106,7 @@ template <int NB> __device__ __forceinline__ void fwd_weights(f32x16 (&s)[NB], f
     }
 }
 
-// One row tile over keys kt0 * BN .. of its sequence.
+// One row tile, which has rows, over keys kt0 * BN .. of its sequence.
 template <typename T, int D, int NW, bool SPLIT>
 __device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* tiles, int h, const Seq& sq, int piece) {
   using F = Frag<T, D>;
@@ -116,8 +116,7 @@ __device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* tiles, int h
   const int b = sq.b, start = sq.start, len = sq.len, k0 = sq.start2, lk = sq.len2;
   const int rows = len * a.G, r0 = sq.tile * BM;
   // rows behind the last sequence belong to nothing: zeros
-  const int store_rows = b == a.B - 1 ? (a.Mq - start) * a.G : rows;
-  if (r0 >= store_rows) return;
+  const int store_rows = b == a.B - 1 ? (a.Mq - start) * a.G : rows;   // (r0 is below it)
   const int off = lk - len;
   int kend = r0 < rows ? lk : 0;
   if (a.causal && kend) kend = max(0, min(lk, group_div(min(r0 + BM, rows) - 1, a.G, a.gmagic) + off + 1));
@@ -232,7 +231,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void packed_fwd_ke
   } else {
     int h, t;
     if (!head_tile(a.d, a.hkv, a.tiles, h, t)) return;
-    const Seq sq = find_tile(a.cu_q, a.cu_k, a.B, a.Mq, a.Mk, a.G, 32 * NW, a.tiles - 1 - t, lane);
+    Seq sq;
+    if (!find_tile(a.cu_q, a.cu_k, a.B, a.Mq, a.Mk, a.G, 32 * NW, a.tiles - 1 - t, lane, sq)) return;
     fwd_rows<T, D, NW, false>(a, tiles, h, sq, 0);
   }
 }

@@ -229,7 +229,7 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal=False, scale=None, return_
     h * G .. h * G + G - 1 share key / value head h).  Row and head strides are free (the column slices of one
     projection's rows need no copy).  cu_q int32 [sequences + 1] on the device: sequence b asks with rows
     cu_q[b] .. cu_q[b+1] - 1 of q; cu_k (default: cu_q) likewise for the keys; offsets begin at 0 and do not
-    decrease, any length may be 0 or 1.  causal: key j is seen by query i where j <= i + keys - queries.  A row
+    decrease (they are not checked: of ones that do the results are unspecified), any length may be 0 or 1.  causal: key j is seen by query i where j <= i + keys - queries.  A row
     that sees no key, and a row behind the last sequence, is 0 (lse -inf) and has zero gradients.
     Returns out [rows, heads, D], with return_lse also the fp32 log-sum-exp [rows, heads] (no gradient).
     A non-finite value in v reaches its own sequence only, also where causal hides it."""

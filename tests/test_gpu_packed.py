@@ -250,6 +250,35 @@ def test_attention_bad_offsets_stay_inside():
     assert torch.equal(got, packed_attention(q, k, v, torch.tensor([0, 10, 40], dtype=torch.int32, device=DEV)))
 
 
+@pytest.mark.parametrize("h,hkv", [(2, 2), (2, 1), (4, 1), (6, 2)])
+@pytest.mark.parametrize("offsets", [(0, 60, 5, 60), (0, 60, *(5,) * 70, 60), (0, 3, 1, 500, -4, 20), (0, *(60, 0) * 40)], ids=lambda o: str(len(o)))
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_decreasing_offsets_stay_inside(h, hkv, offsets, causal):
+    """Offsets that decrease are the caller's error: the results are unspecified, nothing beside them is written."""
+    import ogv._lib as L
+    from ogv import packed as P
+    m, D, edge, boxes = 60, 32, 4096, []
+    q, k, v, do = (t.to(DEV) for t in _qkv(m, m, h, hkv, D, BF, 2))
+    cu = torch.tensor(offsets, dtype=torch.int32, device=DEV)
+
+    def boxed(*shape, dtype=BF):
+        n = math.prod(shape)
+        box = torch.full((n + 2 * edge,), 7.0, dtype=dtype, device=DEV)
+        boxes.append(box)
+        return box[edge:edge + n].view(shape)
+
+    out, lo, dq = (boxed(m, h, D) for _ in range(3))
+    dk, dv = (boxed(m, hkv, D) for _ in range(2))
+    lse = boxed(m, h, dtype=F32)
+    d, ws, _ = P._packed_desc(len(offsets) - 1, m, m, h, hkv, D, causal, D**-0.5, L.OGV_BF16, *(P._strides(t) for t in (q, k, v, out)))
+    ws = P._ws(ws, q)
+    P._launch(L.load().ogv_packed_attn_fwd, "ogv_packed_attn_fwd", q, *map(P._ptr, (q, k, v, cu, cu, out, lo, lse, ws)), d, L.OGV_BF16)
+    P._attn_bwd(do, q, k, v, out, lo, lse, cu, cu, causal, D**-0.5, dq, dk, dv)
+    torch.cuda.synchronize()
+    for box in boxes:
+        assert (box[:edge] == 7).all() and (box[-edge:] == 7).all()
+
+
 def test_attention_no_rows():
     from ogv.packed import packed_attention
     z = torch.zeros(0, 2, 16, device=DEV, requires_grad=True)
