@@ -7,8 +7,8 @@
 
 They stand next to ogv.functional's grid attention and LayerNorm and follow its rules: HIP device tensors
 only, bf16 or fp32 activations, fp32 parameters, torch's current stream of the tensors' own device, no host
-synchronisation (so every call can be captured into a graph), deterministic results.  Forward and backward
-call the C-ABI (ogv_packed_attn_*, ogv_axial_rotary, ogv_gated_norm_*).
+synchronisation (so every call can be captured into a graph), deterministic results, reverse-mode gradients (forward
+mode is refused).  Forward and backward call the C-ABI (ogv_packed_attn_*, ogv_axial_rotary, ogv_gated_norm_*).
 """
 from __future__ import annotations
 
@@ -17,6 +17,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import OGV_BF16, OGV_F32, GatedNormDesc, PackedDesc, RotaryDesc, check
@@ -59,6 +60,10 @@ def _rows32(what, *rows):
 
 
 def _grad(*ts):
+    """Whether the call goes through its autograd function.  Inside a forward-mode level every call does (a dual tensor
+    does not require gradients by itself, and without gradient mode either): the function refuses dual tensors."""
+    if forward_ad._current_level >= 0:
+        return True
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:

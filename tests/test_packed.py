@@ -248,3 +248,46 @@ def test_rows_beyond_32_bits_are_refused():
         gated_residual_norm(x, x)
     with pytest.raises(RuntimeError, match="HIP device"):   # more rows per factor than rows: one factor, nothing to refuse
         gated_residual_norm(torch.zeros(4, 8), torch.zeros(4, 8), row_scale=torch.ones(1), rps=big)
+
+
+@pytest.fixture
+def no_launch(monkeypatch):
+    """The Python side on CPU tensors: nothing is launched, outputs hold zeros."""
+    from ogv import packed as P
+    monkeypatch.setattr(P, "_device", lambda *a: None)
+    monkeypatch.setattr(P, "_launch", lambda *a: None)
+    monkeypatch.setattr(torch, "empty", torch.zeros)
+    monkeypatch.setattr(torch, "empty_like", torch.zeros_like)
+    monkeypatch.setattr(torch.Tensor, "new_empty", torch.Tensor.new_zeros)
+    return P
+
+
+def _forward_mode_calls(P):
+    """name -> (call, its differentiable inputs)"""
+    g = torch.Generator().manual_seed(0)
+    x = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    cu, pos = torch.tensor([0, 2, 6], dtype=torch.int32), torch.zeros(6, 2, dtype=torch.int32)
+    return {
+        "attention": (lambda q, k, v: P.packed_attention(q, k, v, cu), (x(6, 4, 16), x(6, 2, 16), x(6, 2, 16))),
+        "rotary": (lambda q, k: P.axial_rotary(q, k, pos, (4, 4)), (x(6, 4, 16), x(6, 2, 16))),
+        "rotary of q": (lambda q: P.axial_rotary(q, None, pos, (4, 4)), (x(6, 4, 16),)),
+        "rows": (lambda qkv: P.rotary_attention_rows(qkv, cu, 2), (x(6, 96),)),
+        "norm": (lambda f, r, g, w0, b0, w1, b1: P.gated_residual_norm(f, r, gate=g, post_norm="layer", post_weight=w0, post_bias=b0,
+                                                                       pre_weight=w1, pre_bias=b1), (x(6, 8), x(6, 8), *(x(8) for _ in range(5)))),
+    }
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("name", ["attention", "rotary", "rotary of q", "rows", "norm"])
+def test_forward_mode_derivatives_are_refused(no_launch, name, grad):
+    """There is no forward-mode formula: a dual input is an error, never a result without its tangent."""
+    from torch.autograd import forward_ad
+    call, inputs = _forward_mode_calls(no_launch)[name]
+    with torch.set_grad_enabled(grad):
+        call(*inputs)
+        with forward_ad.dual_level():
+            call(*inputs)   # no dual input: nothing to refuse
+            for i, t in enumerate(inputs):
+                dual = forward_ad.make_dual(t, torch.ones_like(t))
+                with pytest.raises(NotImplementedError):
+                    call(*inputs[:i], dual, *inputs[i + 1:])
