@@ -116,7 +116,8 @@ __device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* tiles, int h
   const int b = sq.b, start = sq.start, len = sq.len, k0 = sq.start2, lk = sq.len2;
   const int rows = len * a.G, r0 = sq.tile * BM;
   // rows behind the last sequence belong to nothing: zeros
-  const int store_rows = b == a.B - 1 ? (a.Mq - start) * a.G : rows;   // (r0 is below it)
+  const int store_rows = b == a.B - 1 ? (a.Mq - start) * a.G : rows;
+  if (r0 >= store_rows) return;   // (never: but without it the compiler makes a slower split kernel, 31.2 us for 30.5)
   const int off = lk - len;
   int kend = r0 < rows ? lk : 0;
   if (a.causal && kend) kend = max(0, min(lk, group_div(min(r0 + BM, rows) - 1, a.G, a.gmagic) + off + 1));
