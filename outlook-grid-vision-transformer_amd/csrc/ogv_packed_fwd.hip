@@ -82,15 +82,18 @@ __device__ __forceinline__ float fwd_reference(f32x16 (&s)[NB], f32x16 (&o)[D / 
   }
   const float mz = m == -INFINITY ? 0.f : m;   // nothing visible yet: every weight is exp2(-inf) = 0
   const float mu = mz * c2;
-  // exp2(s * c2 - mu) in one fma: mu's rounding is the same factor in every weight of the row and cancels, unless
-  // it is large itself; then the reference is subtracted first
-  if (__any(fabsf(mu) > 16777216.f)) {
+  // exp2(s * c2 - mu) in one fma: the rounding of mu is the same factor in all weights taken against one reference, and
+  // cancels among them.  When the reference moves, what was summed so far keeps the old one's: a relative 2^-24 |mu|,
+  // which is what the scores themselves are off by.  Where mu is large, a row's reference is subtracted first.
+  const bool far = fabsf(mu) > 16777216.f;
+  if (__any(far)) {
     rare_branch();
+    const float sub = far ? mz : 0.f;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[nb][i] -= mz;
-    return 0.f;
+      for (int i = 0; i < 16; ++i) s[nb][i] -= sub;
+    return far ? 0.f : mu;
   }
   return mu;
 }

@@ -226,6 +226,24 @@ def test_attention_masked_keys_of_any_size():
     assert (out.double().cpu() - mean).abs().max() <= 2.0**-24 * 64 * v.abs().max()
 
 
+@pytest.mark.parametrize("D", [32, 128])
+@pytest.mark.parametrize("dtype", [BF, F32], ids=str)
+def test_attention_rows_decide_for_themselves(dtype, D):
+    """A row of huge or infinite scores (exponents past 2^24) leaves the rows beside it in its tile as they were."""
+    from ogv.packed import packed_attention
+    q, k, v, _ = (t.to(DEV) for t in _qkv(100, 300, 2, 1, D, dtype, D))
+    k[..., 0] = k[..., 0].abs() + 0.5
+    cu_q, cu_k = R.offsets((100,)).to(DEV), R.offsets((300,)).to(DEV)
+    want = packed_attention(q, k, v, cu_q, cu_k, return_lse=True)
+    others = torch.arange(100, device=DEV) != 41
+    for huge in (1e9, -1e9, math.inf):
+        q2 = q.clone()
+        q2[41, 1, 0] = huge
+        got = packed_attention(q2, k, v, cu_q, cu_k, return_lse=True)
+        for a, b in zip(got, want):
+            assert torch.equal(a[others], b[others]) and torch.equal(a[41, 0], b[41, 0])
+
+
 @pytest.mark.parametrize("D", [24, 32, 72])
 @pytest.mark.parametrize("dtype", [BF, F32], ids=str)
 def test_attention_key_of_minus_infinity(dtype, D):
