@@ -164,7 +164,8 @@ __device__ __forceinline__ void fwd_rows(const PackedArgs& a, char* tiles, int h
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) o[db] = f32x16{};
   float m = -INFINITY, l = 0.f;   // m: of q . k, before the scale; l: this lane's half of the row
-  const float c2 = a.scale * LOG2E, grow = 8.f / c2;
+  // (grow is finite, so that the first visible score always moves the reference from -inf, however small the scale)
+  const float c2 = a.scale * LOG2E, grow = fminf(8.f / c2, 3e38f);
 
   if (kt0 < kt1) {
     f32x16 s[NB];

@@ -244,6 +244,23 @@ def test_attention_rows_decide_for_themselves(dtype, D):
             assert torch.equal(a[others], b[others]) and torch.equal(a[41, 0], b[41, 0])
 
 
+@pytest.mark.parametrize("scale", [1e-30, 1.5e-38, 1e-38, 2.0**-140])
+@pytest.mark.parametrize("lq,lk", [((40, 70), (40, 70)), ((1,), (2500,))], ids=str)
+@pytest.mark.parametrize("dtype", [BF, F32], ids=str)
+def test_attention_tiny_scales(dtype, lq, lk, scale):
+    """All weights of a row are equal then, however small the scale: a row that sees keys is never one that sees none."""
+    from ogv.packed import packed_attention
+    q, k, v, do = _qkv(sum(lq), sum(lk), 2, 1, 32, dtype, 3)
+    ts = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+    out, lse = packed_attention(*ts, R.offsets(lq).to(DEV), R.offsets(lk).to(DEV), causal=True, scale=scale, return_lse=True)
+    dq, dk, dv = torch.autograd.grad(out, ts, do.to(DEV))
+    ref = R.attention(q, k, v, lq, lk, True, scale, dtype, do)
+    for got, n in ((out, "out"), (lse, "lse"), (dv, "dv")):
+        _near(got, *ref[n], n)
+    for got, n in ((dq, "dq"), (dk, "dk")):   # below the smallest normal number a result may be flushed to zero
+        _near(got, ref[n][0], ref[n][1] + 2.0**-126, n)
+
+
 @pytest.mark.parametrize("D", [24, 32, 72])
 @pytest.mark.parametrize("dtype", [BF, F32], ids=str)
 def test_attention_key_of_minus_infinity(dtype, D):
