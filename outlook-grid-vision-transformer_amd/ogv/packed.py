@@ -373,7 +373,7 @@ def axial_rotary(q, k, positions, sections, theta=10000.0, interleaved=False):
 
 
 class _RotaryAttentionRows(torch.autograd.Function):
-    """out = attention of the (turned) column slices of qkv; one gradient buffer, written in place."""
+    """out [rows, heads, D] = attention of the (turned) column slices of qkv; one gradient buffer, written in place."""
 
     @staticmethod
     def _split(rows, heads, kv_heads):
@@ -391,7 +391,7 @@ class _RotaryAttentionRows(torch.autograd.Function):
         out, lse = _attn_fwd(q, k, v, cu, cu, causal, scale, lo)
         ctx.save_for_backward(qkv, *((q, k) if rot is not None else (None, None)), out, lo, lse, cu, positions)
         ctx.meta = (rot, heads, kv_heads, causal, scale)
-        return out.flatten(1)
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -402,7 +402,7 @@ class _RotaryAttentionRows(torch.autograd.Function):
         q, k = (q0, k0) if rot is None else (q, k)
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         dq, dk, dv = _RotaryAttentionRows._split(dqkv, heads, kv_heads)
-        _attn_bwd(_heads3(dout.to(qkv.dtype).unflatten(1, (heads, -1))), q, k, v, out, lo, lse, cu, cu, causal, scale, dq, dk, dv)
+        _attn_bwd(_heads3(dout.to(qkv.dtype), heads // kv_heads), q, k, v, out, lo, lse, cu, cu, causal, scale, dq, dk, dv)
         if rot is not None:
             _rotate((dq, dk), (dq, dk), positions, rot, True)
         return dqkv, None, None, None, None, None, None, None
@@ -434,7 +434,7 @@ def rotary_attention_rows(qkv, cu, heads, kv_heads=None, positions=None, section
     al = 16 // qkv.element_size()
     if qkv.stride(1) != 1 or qkv.stride(0) % al or qkv.stride(0) >= 1 << 24 or qkv.data_ptr() % 16:
         qkv = qkv.clone(memory_format=torch.contiguous_format)
-    return _RotaryAttentionRows.apply(qkv, cu, positions, rot, int(heads), kv_heads, bool(causal), scale)
+    return _RotaryAttentionRows.apply(qkv, cu, positions, rot, int(heads), kv_heads, bool(causal), scale).flatten(1)
 
 
 # ------------------------------------------------------------------------------------------------

@@ -291,3 +291,15 @@ def test_forward_mode_derivatives_are_refused(no_launch, name, grad):
                 dual = forward_ad.make_dual(t, torch.ones_like(t))
                 with pytest.raises(NotImplementedError):
                     call(*inputs[:i], dual, *inputs[i + 1:])
+
+
+def test_rows_attention_result_may_be_changed_in_place(no_launch):
+    """As packed_attention's: in-place work on the result is allowed, and a backward that needs the old values says so."""
+    qkv, cu = torch.randn(6, 96, requires_grad=True), torch.tensor([0, 2, 6], dtype=torch.int32)
+    out = no_launch.rotary_attention_rows(qkv, cu, 2)
+    assert out.shape == (6, 32)
+    out += 1.0
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+    (no_launch.rotary_attention_rows(qkv, cu, 2) + 1.0).sum().backward()
+    assert qkv.grad.shape == qkv.shape
