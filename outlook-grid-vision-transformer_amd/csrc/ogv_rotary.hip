@@ -33,7 +33,7 @@ struct RotArgs {
   unsigned char axis[ROT_PAIRS];
 };
 
-// V elements of each half of the pairs (or of interleaved pairs) per item
+// V elements of each half of the pairs (or of interleaved pairs) per item; a workgroup's items are counted in 32 bits
 template <typename T, int V, bool INTER>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs a, int TB) {
   extern __shared__ float2 cs[];   // [TB][P]: cos, sin
@@ -149,7 +149,9 @@ extern "C" int ogv_axial_rotary(const void* q, void* q_out, const void* k, void*
   }
   a.pos = positions, a.M = d->M, a.axes = d->axes, a.D = d->D, a.P = P, a.interleaved = d->interleaved;
   a.pos_float = d->pos_float, a.sign = d->inverse ? -1.f : 1.f;
-  const int TB = 8;
+  const int TB = 8, V = vec ? 8 : d->interleaved ? 2 : 1;
+  const long items = (long)(d->M < TB ? d->M : TB) * ((long)d->heads[0] + d->heads[1]) * ((d->interleaved ? 2 * P : P) / V + (d->D - 2 * P) / V);
+  OGV_REQUIRE(items < (1L << 31) - 256, "ogv_axial_rotary: too many heads (%d + %d)", d->heads[0], d->heads[1]);
   if (dt == OGV_BF16) rotary_launch<bf16>(a, vec, TB, as_stream(stream));
   else rotary_launch<float>(a, vec, TB, as_stream(stream));
   return check_launch("ogv_axial_rotary");

@@ -303,3 +303,19 @@ def test_rows_attention_result_may_be_changed_in_place(no_launch):
         out.sum().backward()
     (no_launch.rotary_attention_rows(qkv, cu, 2) + 1.0).sum().backward()
     assert qkv.grad.shape == qkv.shape
+
+
+@pytest.mark.parametrize("D,pairs,interleaved,M,heads", [(128, 64, 0, 1 << 20, 1 << 25), (128, 64, 1, 8, 1 << 25), (2, 1, 0, 8, 1 << 28),
+                                                         (16, 5, 0, 3, 1 << 26), (16, 4, 0, 1, (1 << 31) - 1)])
+def test_rotary_refuses_more_heads_than_it_can_count(D, pairs, interleaved, M, heads):
+    """A workgroup counts the pieces of its tokens' heads in 32 bits."""
+    import ogv._lib as L
+    lib, x = L.load(), ctypes.c_void_p(64)
+    for split in (0, 5):   # all heads in q, or some of them in k
+        d = L.RotaryDesc(M=M, D=D, axes=1, theta=1e4, interleaved=interleaved)
+        d.heads[0], d.heads[1], d.pairs[0] = heads - split, split, pairs
+        for i in range(2):
+            d.row_in[i] = d.row_out[i] = heads * D
+            d.head_in[i] = d.head_out[i] = D
+        assert lib.ogv_axial_rotary(x, x, x, x, x, ctypes.byref(d), 1, None) == L.OGV_ERR_ARG
+        assert "too many heads" in lib.ogv_last_error().decode()
