@@ -135,14 +135,18 @@ template <int RB> __device__ __forceinline__ Chunk lds_chunk(const char* tile, i
 
 // 16 bytes a lane, from base + off (base uniform) straight to LDS: lane i's to l + 16 * i.  In assembly because the
 // compiler would make every later LDS read wait for the copy, whichever tile it writes; nothing comes back in registers,
-// and tiles_ready() below waits before anybody reads the tile.  (m0 holds the LDS address; its write needs a wait state.
-// Nothing else in these kernels uses m0.)
+// and tiles_ready() below waits before anybody reads the tile.  m0 holds the LDS address; its write needs a wait state.  m0
+// is named as clobbered, so that no write of it by the compiler, for an instruction of its own, is taken to live past the
+// copy (the compiler reserves m0 and warns about that: switched off).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void copy16(const char* base, unsigned off, char* l) {
   const unsigned at = (unsigned)(uint64_t)l;   // an LDS address is the low half of its generic one
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(off),
                "s"(base)
-               : "memory");
+               : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 template <typename P> __device__ __forceinline__ const char* uniform_ptr(const P* p) {
   const uint64_t v = (uint64_t)p;
