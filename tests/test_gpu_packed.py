@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+import _norm_ref as N
 import _packed_ref as R
 
 pytestmark = pytest.mark.gpu
@@ -515,6 +516,32 @@ def test_norm_kinds(post, pre, C):
 def test_norm_samples(M, samples, rs, C):
     """A gate per sample, more samples than workgroups, more rows than a workgroup takes at once."""
     _norm_check(M, C, F32, "rms", "layer", samples=samples, rs=rs)
+
+
+@pytest.mark.parametrize("use", ["both", "y", "h"])
+@pytest.mark.parametrize("c", N.CASES, ids=lambda c: "-".join(str(v).replace("torch.", "") for v in c))
+def test_norm_values_and_gradients(c, use):
+    """Every output and gradient within a bound made of its own terms' roundings (test_norm_bounds.py: broken gradients
+    do not lie within them)."""
+    from ogv.packed import gated_residual_norm
+    M, C, dtype, post, pre, samples, rs, alpha = c
+    t, dy, dh = N.case(M, C, dtype, post, pre, samples, rs)
+    dy, dh = (None if use == "h" and pre else dy), (dh if use != "y" and pre else None)
+    want = N.gated_norm(t, dy, dh, alpha, post, pre, rs or 1)
+    p = {n: None if v is None else v.to(DEV).requires_grad_(n != "rs") for n, v in t.items()}
+    out = gated_residual_norm(p["f"], p["x"], gate=p["gate"], row_scale=p["rs"], rps=rs or 1, alpha=alpha, post_norm=post, post_weight=p["post_w"],
+                              post_bias=p["post_b"], pre_norm=pre, pre_weight=p["pre_w"], pre_bias=p["pre_b"])
+    y, h = out if pre else (out, None)
+    wrt = [n for n, v in p.items() if v is not None and n != "rs"]
+    outs = [(o, g.to(DEV)) for o, g in ((y, dy), (h, dh)) if g is not None]
+    got = dict(zip(wrt, torch.autograd.grad([o for o, _ in outs], [p[n] for n in wrt], [g for _, g in outs])))
+    got.update(y=y, **({"h": h} if pre else {}))
+    for n, g in got.items():
+        if n not in want:   # (no gradient reaches the pre norm without dh)
+            assert (g == 0).all(), n
+            continue
+        assert g.shape == want[n].x.shape and g.dtype == (dtype if n in "yhfx" else F32)
+        assert N.excess(g, want[n], g.dtype) <= 0, n
 
 
 @pytest.mark.parametrize("use", [("y",), ("h",)])
