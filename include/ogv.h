@@ -214,7 +214,8 @@ int ogv_layernorm_bwd(const void* dy, const void* x, const float* gamma, const f
  * Backward: dout, dq like q; dk, dv like k; out, out_lo (NULL: taken as 0) and lse as the forward wrote them.
  * ws >= the *_ws_bytes query (forward: 0 bytes, may be NULL, unless the keys are split).  Deterministic.
  * The backward forms the weights again from lse in fp32: a weight's relative error is about 2^-23 |scale q . k|.
- * A non-finite value in v reaches its own sequence only.  bf16 or fp32, D % 8 == 0, D <= 128, scale > 0.
+ * A non-finite value in v reaches its own sequence only, also where causal hides it; so does, in the backward, one in
+ * q, k, v or dout (a weight of 0 times it is not 0).  bf16 or fp32, D % 8 == 0, D <= 128, scale > 0.
  * ------------------------------------------------------------------------------------------- */
 #define OGV_PACKED_TENSORS 8
 typedef struct {

@@ -10,10 +10,13 @@
 //   N'(g) = rstd (g w - [mean(g w)] - vhat mean(g w vhat))        ([.]: layer only)
 //
 // Bound by memory: forward f, x -> y, h (4 rows of C), backward f, x, dy, dh -> df, dx (6): 65536 rows of 768, bf16, layer
-// norms on both sides take 90 us and 133 us, 4.5 TB/s (a large copy: 4.9); 12800 rows of 331, fp32, 15 and 26 us.  The
-// backward loads the next row while it works on one (with it and two sums for three gradients: 355 -> 133 us, as the
-// registers then leave two waves to a SIMD).  A row belongs to
-// G lanes (a part of a wave, a wave, or a workgroup) that keep it in registers through every reduction.
+// norms on both sides take 90 us and 133 us, 4.5 TB/s (a large copy: 4.9); 12800 rows of 331, fp32, 15 and 26 us; wider
+// rows were not timed.  The backward loads the next row while it works on one.  A row belongs to G lanes (a part of a
+// wave, a wave, or a workgroup) that hold it through every reduction, in registers as far as these go.  Of rows above 512
+// channels read in vectors, the backward's registers leave two waves to a SIMD at 520 to 768 in bf16 with a gate per
+// channel (which, with two sums for three gradients, took the case above from 355 to 133 us) and at 1032 to 2048, else one.
+// Above 4096 channels it spills: 97 registers (bf16) or 224 (fp32), 221 or 343 with a gate per sample, 515 to 631 where
+// single columns are read.
 // Column sums: each lane adds its columns over the workgroup's rows, one partial row per workgroup, then they are added
 // in a fixed order: no atomics.
 #include "ogv_common.h"

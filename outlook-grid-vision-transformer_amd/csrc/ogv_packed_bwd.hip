@@ -13,9 +13,10 @@
 //
 // Measured on one MI355X: D = 128, causal, 16 heads on 4, sequences of 4096 and 2451 (327 GFLOP with the forward): dq 177 us
 // (791 TFLOP/s of its three products), dk / dv 259 us (722, four products) and 23 us to add its row pieces.  Both are
-// bound by the matrix instructions and the LDS reads that feed them (24 and 40 KB a 32x32 block of scores).  D = 64, 64
-// images of 49 to 784 tokens, 6 heads: dq 56 us and dk / dv 59 us, of which 22 and 16 are the workgroups' ends (rows read
-// and written); 5 tiles a workgroup do not hide the rest.
+// bound by the matrix instructions and the LDS reads that feed them (24 and 40 KB a 32x32 block of scores); dk / dv has all
+// 256 registers of two waves a SIMD taken and 10 more in scratch.  D = 64, 64 images of 49 to 784 tokens, 6 heads: dq 55 us
+// and dk / dv 58 us, of which 22 and 16 are the workgroups' ends (rows read and written); 5 tiles a workgroup do not hide the
+// rest.  dq's keys are never split: with one query a sequence, its few waves walk all of them.
 #include "ogv_packed.h"
 
 #include <initializer_list>
@@ -341,7 +342,7 @@ struct BwdPlan {
 
 // Waves per workgroup as in the forward.  The rows of dk / dv are split while the key tiles would not fill the 256 CUs
 // twice, into 1024 workgroups or a few more (two to a CU, twice: under the causal mask the first tile has twice the
-// average work; long causal streams, D = 128: with 768 the step takes 1.06, with 1536 1.04 times as long).  A piece costs
+// average work; measured on long causal streams, D = 128, alone: with 768 the step takes 1.06, with 1536 1.04 times as long).  A piece costs
 // 16 bytes of partial sums per key, head and dim, so it has at least 512 rows on average, 32 in fp32, whose products run
 // at a sixteenth of the rate.
 static BwdPlan bwd_plan(const ogv_packed_desc* d, ogv_dtype dt) {

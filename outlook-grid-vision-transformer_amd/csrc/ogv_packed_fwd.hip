@@ -12,17 +12,20 @@
 // large).  For a backward, what rounding took from o is kept too (out_lo): see delta there.
 //
 // Split: four waves of 32 rows share the tiles (64 keys; 32 in fp32 and for one-wave workgroups of short sequences), two
-// workgroups to a CU for D = 128, three for D = 64.  A row tile's keys are walked in one piece where the row tiles fill
-// the chip; otherwise (single queries) they are cut into equal pieces whose partial results a second kernel joins.
+// workgroups to a CU for D = 128, three for D = 64.  A row tile's keys are walked in one piece where there are row tiles
+// enough for two to a CU; where there are fewer (single queries) they are cut into equal pieces whose partial results a
+// second kernel joins.  The host decides by the numbers of rows, keys and sequences alone (the lengths are on the device):
+// one long sequence among hundreds of short ones is walked by the waves that suit those, in one piece.
 //
 // What bounds it, measured on one MI355X (a large bf16 matrix product reaches 1365 TFLOP/s):
-//   D = 128, causal, 16 heads on 4, sequences of 8191 and 5608: 405 us, 996 TFLOP/s.  Left out in turn, the first product
-//     saves 116 us, the second 133, the copies to LDS 61, the exponentials 7: the matrix instructions and the LDS reads that
-//     feed them (1 KB a product of 32 cycles, half the LDS rate from two waves a SIMD) do not overlap further.
-//   D = 64, 48 images of 196 to 1024 tokens, 12 heads: 91 us, 540 TFLOP/s.  29 us of it are the workgroups' ends (q read, out
-//     written: 78 MB), the rest is spread over the 16-cycle exponentials (42 us for all of them with the other vector
-//     instructions) and the latencies of 3 to 16 tiles a workgroup.
-//   One query for each of 64 sequences (up to 8192 keys), 16 heads on 2: 30.8 us for 100 MB of keys and values, 3.2 TB/s, of
+//   D = 128, causal, 16 heads on 4, sequences of 8191 and 5608: 405 to 411 us from box to box, 980 to 1000 TFLOP/s.  Left out
+//     in turn (of 423 us then), the first product saved 117 us, the second 133, the copies to LDS 62, the exponentials 7: the
+//     matrix instructions and the LDS reads that feed them (1 KB a product of 32 cycles, half the LDS rate from two waves a
+//     SIMD) do not overlap further.
+//   D = 64, 48 images of 196 to 1024 tokens, 12 heads: 92 to 95 us, 520 to 535 TFLOP/s.  29 us of it are the workgroups' ends
+//     (q read, out written: 78 MB), the rest is spread over the 16-cycle exponentials (42 us for all of them with the other
+//     vector instructions, by their count) and the latencies of 3 to 16 tiles a workgroup.
+//   One query for each of 64 sequences (up to 8192 keys), 16 heads on 2: 30.7 us for 100 MB of keys and values, 3.3 TB/s, of
 //     which the joining launch takes 5.
 // The next tile's scores are computed before this tile's exponentials (466 -> 431 us at D = 128), copies bypass the
 // registers (1318 -> 558), the reference of the weights moves lazily, heads are dealt evenly to the XCDs (558 -> 479).
@@ -285,9 +288,10 @@ struct FwdPlan {
   unsigned grid;
 };
 
-// Sequences that fill four waves' rows on average get them, others one wave per workgroup.  While the row tiles
-// would not fill the 256 CUs twice, the keys are split into pieces of equal size (not equal number: sequences
-// differ), about 800 in all (64 single queries, 97 thousand keys, 16 heads on 2 of 128: 30.8 us; 1024 31.5, 1500 32.9).
+// Sequences that fill four waves' rows on average get them, others one wave per workgroup.  While there are fewer than
+// 512 row tiles and at least two pieces of keys to a sequence on average, the keys are split into pieces of equal size (not
+// equal number: sequences differ), about 800 in all (measured at one shape, 64 single queries, 97 thousand keys, 16 heads
+// on 2 of 128: 30.8 us; 1024 pieces 31.5, 1500 32.9).
 static FwdPlan fwd_plan(const ogv_packed_desc* d) {
   FwdPlan p;
   const long rows = (long)d->Mq * (d->heads / d->kv_heads);

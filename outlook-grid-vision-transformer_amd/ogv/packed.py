@@ -237,7 +237,8 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal=False, scale=None, return_
     decrease (they are not checked: of ones that do the results are unspecified), any length may be 0 or 1.  causal: key j is seen by query i where j <= i + keys - queries.  A row
     that sees no key, and a row behind the last sequence, is 0 (lse -inf) and has zero gradients.
     Returns out [rows, heads, D], with return_lse also the fp32 log-sum-exp [rows, heads] (no gradient).
-    A non-finite value in v reaches its own sequence only, also where causal hides it."""
+    A non-finite value in v reaches its own sequence only, also where causal hides it; so does, in the backward, one
+    in q, k, v or the gradient (a weight of 0 times it is not 0)."""
     what = "ogv.packed_attention"
     dt = _dtype(what, q, k, v)
     causal, scale = bool(causal), None if scale is None else float(scale)
